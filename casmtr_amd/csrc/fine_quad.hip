@@ -354,7 +354,7 @@ __global__ __launch_bounds__(128, (NPASS == 1 ? 4 : 3)) void fine_quad_kernel(co
     auto prefetch = [&](const Item& it, int buf) {   // 1 DMA instruction
         const unsigned qd = (unsigned)((it.b * H + h) * Lq + it.quad), bq = (unsigned)(it.b * Lq + it.quad);   // wave-uniform
         const unsigned long long addr = sbase + (unsigned long long)qd * mulq + (unsigned long long)bq * mula;
-        const unsigned dst = stg_lds + (unsigned)(buf * STG * 4);
+        const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane((int)(stg_lds + (unsigned)(buf * STG * 4)));   // an SGPR for M0, whatever the compiler can prove
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(addr), "s"(dst) : "memory");
         if ((Kp & 3) && lane < 32) {   // a 16-byte read of the last list piece would run past the table's end: 4-byte pieces, lanes 0-31 only
             const unsigned off = qd * (unsigned)(Kp * 4) + (unsigned)(min(lane, Kp - 1) * 4);
