@@ -7,6 +7,7 @@ to the CPU.
 """
 from __future__ import annotations
 
+import math
 import os
 
 import torch
@@ -747,3 +748,166 @@ def nms_select(next_conf01, next_idx01, next_idx10, hw0, hw1, nms_window=5, test
                                            _stream()),
                    "nms_select_fwd")
     return dict(b_ids=bi, i_ids=ii, j_ids=ji, mconf=mc, n=n, keep_ws=ws)
+
+
+# ------------------------------------------------------------------------------------------------ packed tokens
+_TOKEN_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_QUANT_TYPES = {torch.float8_e4m3fn: 1, torch.float8_e5m2: 2, torch.int8: 3}
+
+
+def _chk_tok(t, name, like=None, rows=False):
+    """a token tensor: on the device, fp32 / fp16 / bf16, last axis contiguous; `like`: same device and type as that one"""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA (HIP) tensor")
+    if t.dtype not in _TOKEN_TYPES:
+        raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise RuntimeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RuntimeError(f"{name} must be contiguous along its last axis")
+    return t
+
+
+def _rows(t, name):
+    """[..., C] as (rows, C, row stride): the leading axes must collapse to one stride"""
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise RuntimeError(f"{name} must be [..., C] with C >= 1")
+    try:
+        v = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+    except RuntimeError:
+        raise RuntimeError(f"{name}: its leading axes must have one common row stride (a view of rows), got strides {t.stride()}") from None
+    return v.shape[0], v.shape[1], v.stride(0)
+
+
+def _norm_args(x, weight, residual):
+    _chk_tok(x, "x"), _chk_tok(residual, "residual", x), _chk_tok(weight, "weight")
+    if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32) or weight.dim() != 1 or not weight.is_contiguous():
+        raise RuntimeError(f"weight must be a contiguous vector of {x.dtype} or float32 on {x.device}")
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError("residual must have x's shape")
+    R, C, xs = _rows(x, "x")
+    if weight.numel() != C:
+        raise RuntimeError(f"weight must have {C} elements, got {weight.numel()}")
+    return R, C, xs, (0 if residual is None else _rows(residual, "residual")[2])
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None, want_rstd=False):
+    """Root-mean-square norm over the last axis of x [..., C] (fp32 / fp16 / bf16, C <= 16384; rows may be strided):
+        h = round(x + residual);  y = h / sqrt(mean(h^2) + eps) * weight            (weight [C]: x's type or fp32)
+    -> (y, h) -- h is the stream for the next residual, None without a residual --, with want_rstd (y, h, rstd fp32 [rows])."""
+    R, C, xs, rs = _norm_args(x, weight, residual)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = torch.empty_like(y) if residual is not None else None
+    rstd = torch.empty(R, device=x.device, dtype=torch.float32) if want_rstd else None
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().casmtr_rms_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(y), _ptr(h), _ptr(rstd), None, R, C, xs, rs, float(eps),
+                                                  _TOKEN_TYPES[x.dtype], _TOKEN_TYPES[weight.dtype], 0, 0, _stream()), "rms_norm_fwd")
+    return (y, h, rstd) if want_rstd else (y, h)
+
+
+def rms_norm_quant(x, weight, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn, group=None):
+    """rms_norm with the output in 8 bits (float8_e4m3fn, float8_e5m2 or int8), ready for a scaled product:
+        scale = max(max|y| / top, 2^-126);  q = round(y / scale), saturating             (top 448, 57344, 127)
+    with one scale per row (group=None: scale [...]) or per 128 columns (group=128, C % 128 == 0: scale [..., C / 128]).  The maximum is
+    of y in fp32.  -> (q [..., C], scale fp32, h or None)."""
+    if dtype not in _QUANT_TYPES:
+        raise RuntimeError(f"rms_norm_quant: dtype must be one of {[str(t) for t in _QUANT_TYPES]}, got {dtype}")
+    R, C, xs, rs = _norm_args(x, weight, residual)
+    if group is not None and (group != 128 or C % 128):
+        raise RuntimeError(f"rms_norm_quant: group must be None or 128 with C % 128 == 0, got group {group} and C {C}")
+    q = torch.empty(x.shape, device=x.device, dtype=dtype)
+    scale = torch.empty(x.shape[:-1] if group is None else (*x.shape[:-1], C // 128), device=x.device, dtype=torch.float32)
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().casmtr_rms_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(q), _ptr(h), None, _ptr(scale), R, C, xs, rs, float(eps),
+                                                  _TOKEN_TYPES[x.dtype], _TOKEN_TYPES[weight.dtype], _QUANT_TYPES[dtype], group or 0, _stream()),
+                   "rms_norm_fwd")
+    return q, scale, h
+
+
+def rms_norm_bwd(dy, h, weight, rstd, dh=None):
+    """Gradient of rms_norm: h [..., C] (x + residual as returned, or x), rstd from want_rstd, dh the gradient that reaches h from
+    further on -> (dx [..., C], dweight [C]); dx is the gradient of x and of the residual.  The weight's sums have a fixed order."""
+    R, C, hs, _ = _norm_args(h, weight, None)
+    _chk_tok(dy, "dy", h), _chk_tok(dh, "dh", h), _chk(rstd, "rstd")
+    if dy.shape != h.shape or (dh is not None and dh.shape != h.shape) or rstd.numel() != R or rstd.device != h.device:
+        raise RuntimeError("rms_norm_bwd: dy and dh must have h's shape, rstd one value per row")
+    dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    if R == 0:
+        return dx, torch.zeros_like(weight)
+    dw = torch.empty_like(weight)
+    l = _lib.lib()
+    ws = torch.empty(l.casmtr_rms_norm_bwd_ws_floats(R, C), device=h.device, dtype=torch.float32)
+    with torch.cuda.device(h.device):
+        _lib.check(l.casmtr_rms_norm_bwd(_ptr(dy), _ptr(dh), _ptr(h), _ptr(weight), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws), R, C, _rows(dy, "dy")[2],
+                                         0 if dh is None else _rows(dh, "dh")[2], hs, _TOKEN_TYPES[h.dtype], _TOKEN_TYPES[weight.dtype], _stream()),
+                   "rms_norm_bwd")
+    return dx, dw
+
+
+def rotary_freqs(dim, base=10000.0, factor=1.0, trained=None, axes=1, device="cuda"):
+    """Table for ops.rotary: (inv_freq fp64 [dim / 2], gain).  dim: the columns that rotate; axes=2: half of them by the row and half by
+    the column of an image token.  Pair i of an axis' n turns by position * base^(-i / n).
+    factor > 1 stretches the positions for contexts `factor` times longer than trained:
+      trained=None     every frequency is divided by the factor (linear interpolation of positions), gain 1
+      trained=length   frequencies with more than 32 turns over the trained length stay, those with less than one are divided by the
+                       factor, in between they are blended linearly in the number of turns; gain 0.1 ln(factor) + 1"""
+    if dim <= 0 or axes not in (1, 2) or dim % (2 * axes):
+        raise RuntimeError(f"rotary_freqs: dim must be a positive multiple of 2 * axes and axes 1 or 2, got dim {dim}, axes {axes}")
+    if not base > 0 or not factor >= 1 or (trained is not None and not trained > 0):
+        raise RuntimeError(f"rotary_freqs: base > 0, factor >= 1 and trained > 0, got {base}, {factor}, {trained}")
+    n = dim // 2 // axes
+    f = float(base) ** (-torch.arange(n, dtype=torch.float64) / n)
+    gain = 1.0
+    if trained is None:
+        f = f / factor
+    elif factor > 1:
+        keep = ((trained * f / (2 * math.pi) - 1.0) / 31.0).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        gain = 0.1 * math.log(factor) + 1.0
+    return torch.cat([f] * axes).to(device), gain
+
+
+def _chk_heads(t, name, like=None):
+    """[T, H, D] token tensor whose heads are contiguous rows -> (token stride, head stride)"""
+    _chk_tok(t, name, like)
+    if t.dim() != 3:
+        raise RuntimeError(f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
+    return t.stride(0), t.stride(1)
+
+
+def rotary(q, k, positions, inv_freq, layout="half", gain=1.0, inverse=False):
+    """Rotary positions of q [T,Hq,D] and k [T,Hk,D] (k may be None) in one launch -> (q', k').
+    positions: int32 / int64 [T], or [T,2] (row and column of an image token: the first half of the pairs turns by the row, the rest by the
+    column); inv_freq: fp64 [n] on the device, 2 n <= D (rotary_freqs); the first 2 n columns of each head turn, in pairs (i, i + n)
+    (layout 'half') or (2i, 2i + 1) ('interleaved'), the others are copied.
+        (a, b) -> gain * (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq, reduced in 64 bits
+    inverse: t -> -t (the gradient).  q and k may be views with any token and head strides (column ranges of a fused projection)."""
+    if layout not in ("half", "interleaved"):
+        raise RuntimeError(f"rotary: layout must be 'half' or 'interleaved', got {layout!r}")
+    qs = _chk_heads(q, "q")
+    T, Hq, D = q.shape
+    ks, Hk = (0, 0), 0
+    if k is not None:
+        ks, Hk = _chk_heads(k, "k", q), k.shape[1]
+        if k.shape[0] != T or k.shape[2] != D:
+            raise RuntimeError("rotary: q and k must share tokens and head dimension")
+    _chk(inv_freq, "inv_freq", torch.float64)
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"positions must be int32 or int64, got {positions.dtype}")
+    _chk(positions, "positions", positions.dtype)
+    n = inv_freq.numel()
+    axes = 2 if positions.dim() == 2 else 1
+    if inv_freq.dim() != 1 or positions.device != q.device or inv_freq.device != q.device or tuple(positions.shape) not in ((T,), (T, 2)):
+        raise RuntimeError("rotary: positions must be [T] or [T,2] and inv_freq a vector, on q's device")
+    if n < 1 or 2 * n > D or n > 1024 or (axes == 2 and n % 2):
+        raise RuntimeError(f"rotary: 1 to min(D / 2, 1024) pairs (an even number with two positions per token), got {n} for D {D}")
+    oq = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
+    ok = torch.empty((T, Hk, D), device=q.device, dtype=q.dtype) if k is not None else None
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().casmtr_rotary_fwd(_ptr(q), _ptr(k), _ptr(positions), _ptr(inv_freq), _ptr(oq), _ptr(ok), T, Hq, Hk, D, n, axes,
+                                                int(positions.dtype == torch.int64), int(layout == "interleaved"), float(gain), int(bool(inverse)),
+                                                *qs, *ks, _TOKEN_TYPES[q.dtype], _stream()), "rotary_fwd")
+    return oq, ok

@@ -314,6 +314,36 @@ int casmtr_pola_attn_fwd(const float* q, const float* k0, const float* v0, const
                          int nhead, int head_dim, int ws, float scale, casmtr_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * Operators on packed tokens (no reference counterpart): RMS norm, rotary positions, attention over sequences of different
+ * lengths.  Element types are given by code; values are widened to fp32 when loaded and rounded once when stored.  Strides are in
+ * ELEMENTS; the last axis is contiguous.
+ * ---------------------------------------------------------------------------------------------------------- */
+enum { CASMTR_F32 = 0, CASMTR_F16 = 1, CASMTR_BF16 = 2 };
+enum { CASMTR_Q_NONE = 0, CASMTR_Q_E4M3 = 1, CASMTR_Q_E5M2 = 2, CASMTR_Q_I8 = 3 };
+
+/* Root-mean-square norm of `rows` rows of C <= 16384 columns, after the residual's addition where residual != NULL:
+ *   h = round(x + residual) (written to h [rows,C]; without a residual h = x and nothing is written);  rstd = 1 / sqrt(mean(h^2) + eps);
+ *   y = h * rstd * w.  quant == 0: y [rows,C] in `dtype`.  Otherwise y holds 8-bit codes (e4m3, e5m2 or signed integers) of y / scale,
+ *   scale = max(max|y| / top, 2^-126) (top 448, 57344, 127), one scale per row (group == 0: scale [rows]) or per 128 columns
+ *   (group == 128, C % 128 == 0: scale [rows,C/128]).  rstd [rows] is written where not NULL (the gradient takes it).
+ * x_stride / r_stride: distance of two rows.  w_dtype: dtype or CASMTR_F32.                                                  */
+int casmtr_rms_norm_fwd(const void* x, const void* residual, const void* w, void* y, void* h, float* rstd, float* scale, long long rows, int C,
+                        long long x_stride, long long r_stride, float eps, int dtype, int w_dtype, int quant, int group, casmtr_stream_t stream);
+/* Its gradient: g = dy w, n = h rstd;  dx = (g - n mean(g n)) rstd (+ dh where dh != NULL) [rows,C] -- the gradient of x and of the
+ * residual;  dw [C] (in w_dtype) = sum over the rows of dy n, in a fixed order.  rows >= 1.  ws: casmtr_rms_norm_bwd_ws_floats() floats.       */
+size_t casmtr_rms_norm_bwd_ws_floats(long long rows, int C);
+int casmtr_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* ws, long long rows,
+                        int C, long long dy_stride, long long dh_stride, long long h_stride, int dtype, int w_dtype, casmtr_stream_t stream);
+
+/* Rotary positions of q [T,Hq,D] and k [T,Hk,D] (Hk == 0: q alone) -> oq, ok (contiguous): the pairs of a head's first 2 npairs columns turn by
+ * position * inv_freq[pair] (fp64 [npairs], radians; inverse: by minus that) and are scaled by gain, the other columns are copied.
+ * pos [T,axes], int32 or int64; axes == 2: the first half of the pairs takes the first position, the rest the second.  npairs <= 1024. */
+enum { CASMTR_ROTARY_HALF = 0, CASMTR_ROTARY_INTERLEAVED = 1 };
+int casmtr_rotary_fwd(const void* q, const void* k, const void* pos, const double* inv_freq, void* oq, void* ok, long long T, int Hq, int Hk, int D,
+                      int npairs, int axes, int pos_is_i64, int layout, float gain, int inverse, long long q_token_stride, long long q_head_stride,
+                      long long k_token_stride, long long k_head_stride, int dtype, casmtr_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * Measurement hooks (no reference counterpart): per-kernel launch durations from HIP events recorded on the
  * launch stream.  Off by default.  casmtr_prof_enable(1) starts a fresh collection; casmtr_prof_read() waits for
  * the recorded events and returns the summed duration (ms) and the number of launches of kernel `id`.
