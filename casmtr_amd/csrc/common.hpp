@@ -226,9 +226,8 @@ int* work_counters(hipStream_t stream);
 __device__ __forceinline__ void work_claim_issue(int* ctr, bool doit, int& ret) {
     const int m = __builtin_amdgcn_readfirstlane(doit ? 1 : 0);   // (the compiler cannot always prove `doit` uniform: pin it to an SGPR)
     unsigned long long save;
-    const int zero = 0, one = 1;
     asm volatile("s_mov_b64 %1, exec\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, 0\n\tglobal_atomic_add %0, %3, %4, %5 sc0\n\ts_mov_b64 exec, %1"
-                 : "=v"(ret), "=&s"(save) : "s"(m), "v"(zero), "v"(one), "s"(ctr) : "memory");
+                 : "=v"(ret), "=&s"(save) : "s"(m), "v"(0), "v"(1), "s"(ctr) : "memory");
 }
 __device__ __forceinline__ int work_claimed(const int& ret) {   // lane 0's value, wave-uniform
     int s;

@@ -1,0 +1,264 @@
+// Attention over packed sequences of different lengths, forward:
+//   o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j) over the keys j that row i sees,  lse_i = log sum_j exp(scale q_i . k_j)
+// Row i of a sequence with nq rows and nk keys sees all keys, or, causal, the keys j <= i + nk - nq.  A row that sees none gives 0 and -inf.
+// Query heads share key heads in groups of G = H / Hk.
+//
+// One pass over the keys with the running maximum and sum of the softmax.  A tile's rows are (token, head of the group) pairs, token-major, so
+// all G heads of a key head use one copy of its keys, and a single token of G heads is one tile.  A workgroup has four waves of 32 rows; K and V
+// tiles of BN keys go through LDS, the next tile's loads in flight while this one is multiplied.
+#include "packed_attn.hpp"
+
+using namespace casmtr;
+
+namespace {
+struct AttnArgs {
+    const void *q, *k, *v;
+    void* o;
+    float* lse;                        // [Tq, H] or NULL
+    float *part_o, *part_ml;           // splits > 1: [splits, Tq * H, D] and [splits, Tq * H, 2]
+    PackedSeqs s;
+    long long qts, qhs, kts, khs, vts, vhs;   // token and head strides, in elements
+    int H, Hk, D, splits;
+    float scale;                       // times log2(e): scores are in bits
+};
+
+constexpr float LN2 = 0.693147180559945309f;
+constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a maximum grew by more than 8 bits: exp2 stays below 256, far from any overflow
+
+template <typename T, int DP, int BN, int NW>
+__global__ __launch_bounds__(64 * NW) void packed_attn_kernel(const AttnArgs a) {
+    typedef Tile<T, DP> L;
+    constexpr int BM = 32 * NW, NT = 64 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
+    constexpr int NCH = BN * L::CPR / NT;           // chunks per thread of a K (V) tile
+    constexpr int TB = BN * L::RB;                  // bytes of a tile
+    __shared__ __attribute__((aligned(256))) char smem[4 * TB];   // K, V of two stages
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, r = lane & 31;
+    const int hk = blockIdx.x % a.Hk, G = a.s.G;
+    int tile;
+    const int seq = seq_of_slot(a.s.cu_q, a.s.n, a.s.Tq, G, BM, (long long)(gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk), &tile);   // later rows see more keys: first
+    const Span rows = span_of(a.s.cu_q, seq, a.s.n, a.s.Tq), keys = keys_of(a.s, seq);
+    const int nrow = rows.count * G;
+    if ((long long)tile * BM >= nrow) return;   // a slot too many
+    const int row0 = tile * BM;
+    const int row = row0 + 32 * wave + r, rc = min(row, nrow - 1), tok = rc / G, head = hk * G + rc % G;
+    const int shift = keys.count - rows.count;
+    const int limit = a.s.causal ? max(0, min(keys.count, tok + shift + 1)) : keys.count;   // this lane's row sees the keys [0, limit)
+    // keys that some row of the workgroup / of the wave sees (rows see more the later they are), keys that all rows of the wave see
+    const auto limit_at = [&](int rr) { return a.s.causal ? max(0, min(keys.count, min(rr, nrow - 1) / G + shift + 1)) : keys.count; };
+    const int wg_end = limit_at(row0 + BM - 1), wave_end = limit_at(row0 + 32 * wave + 31), wave_all = limit_at(row0 + 32 * wave);
+    int t0 = 0, t1 = (wg_end + BN - 1) / BN;
+    if (a.splits > 1) {
+        const int per = (t1 + a.splits - 1) / a.splits;
+        t0 = min(t1, per * (int)blockIdx.y);
+        t1 = min(t1, t0 + per);
+    }
+    frag_t<T> qf[KS];
+    {
+        const T* qr = (const T*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = load_frag(qr, s, h, a.D);
+    }
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+
+    const T* kb = (const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs;
+    const T* vb = (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs;
+    u32x4 kr[NCH], vr[NCH];
+    const auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int id = tid + NT * i, rr = t * BN + id / L::CPR, c = (id % L::CPR) * L::EPC;
+            kr[i] = u32x4{0, 0, 0, 0};
+            vr[i] = u32x4{0, 0, 0, 0};
+            if (rr < keys.count && c < a.D) {
+                kr[i] = load_chunk(kb + (long long)rr * a.kts, c, a.D);
+                vr[i] = load_chunk(vb + (long long)rr * a.vts, c, a.D);
+            }
+        }
+    };
+    const auto put = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
+            *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = kr[i];
+            *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = vr[i];
+        }
+    };
+    if (t0 < t1) { fetch(t0); put(0); }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int stage = (t - t0) & 1;
+        if (t + 1 < t1) fetch(t + 1);
+        const char *ks = smem + 2 * stage * TB, *vs = ks + TB;
+        if (t * BN < wave_end) {
+            f32x16 s[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                s[b] = zero16();
+#pragma unroll
+                for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, 32 * b + r, st, h), qf[st], s[b]);
+            }
+            const bool hidden = (t + 1) * BN > wave_all;
+            if (hidden) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[b][i] = -INFINITY;
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+            mx = max_halves(mx) * a.scale;
+            const bool up = mx > m + RESCALE_AT;   // (also the first tile: m = -inf); per row, so that a row's bits do not depend on its neighbours
+            if (__any(up)) {
+                const float f = !up ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+                m = up ? mx : m;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+            }
+            const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.scale, -mm));
+                    l += s[b][i];
+                }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    const frag_t<T> p = to_frag<T>(s[b], tt);   // probabilities below 256 rounded to the values' type; l sums the unrounded ones
+                    const int k0 = 32 * b + 16 * tt;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const frag_t<T> vt = L::cols(vs, k0, 32 * d, lane);
+                        if (!hidden) acc[d] = mma(vt, p, acc[d]);
+                        else acc[d] = mma_hidden<T>(vt, p, acc[d], h, [&](int n) { return t * BN + k0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3) < limit; });
+                    }
+                }
+        }
+        if (t + 1 < t1) put(stage ^ 1);
+        __syncthreads();
+    }
+    l = add_halves(l);
+    if (row >= nrow) return;
+    const long long out_row = (long long)(rows.begin + tok) * a.H + head;
+    if (a.splits > 1) {
+        float* po = a.part_o + ((long long)blockIdx.y * a.s.Tq * a.H + out_row) * a.D;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * d + 8 * g + 4 * h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < a.D) po[c + e] = acc[d][4 * g + e];
+            }
+        if (h == 0) {
+            float* ml = a.part_ml + 2 * ((long long)blockIdx.y * a.s.Tq * a.H + out_row);
+            ml[0] = m;
+            ml[1] = l;
+        }
+        return;
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    T* orow = (T*)a.o + out_row * a.D;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * d + 8 * g + 4 * h;
+            typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            T4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[d][4 * g + e] * inv);
+            if (c + 4 <= a.D) *reinterpret_cast<T4*>(orow + c) = v;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < a.D) orow[c + e] = v[e];
+        }
+    if (a.lse && h == 0) a.lse[out_row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+}
+
+// joins the splits of a row: weights 2^(m_s - max m); one wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnArgs a) {
+    const long long rows = a.s.Tq * a.H, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
+    for (int s = 0; s < a.splits; ++s) {
+        const float ms = a.part_ml[2 * (s * rows + row)], ls = a.part_ml[2 * (s * rows + row) + 1];
+        const float f = ms == -INFINITY ? (ls != ls ? ls : 0.f) : __builtin_amdgcn_exp2f(ms - m);
+        if (f == 0.f) continue;   // a split that sees no key
+        const float* po = a.part_o + (s * rows + row) * a.D;
+        l += f * ls;
+        if (lane < a.D) o0 += f * po[lane];
+        if (lane + 64 < a.D) o1 += f * po[lane + 64];
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    T* orow = (T*)a.o + row * a.D;
+    if (lane < a.D) orow[lane] = (T)(o0 * inv);
+    if (lane + 64 < a.D) orow[lane + 64] = (T)(o1 * inv);
+    if (a.lse && lane == 0) a.lse[row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+}
+
+constexpr int FWD_NW = 4;
+
+// How many parts a sequence's keys are split into: enough workgroups to fill the chip when there are few rows.  A part is no shorter than 256 keys on
+// average, so that what it writes (a row of fp32 per query row) stays small beside what it reads.
+int split_count(long long Tq, long long Tk, int n, int H, int Hk) {
+    const long long wgs = ((Tq * (H / Hk) + 32 * FWD_NW - 1) / (32 * FWD_NW) > n ? (Tq * (H / Hk) + 32 * FWD_NW - 1) / (32 * FWD_NW) : n) * Hk;
+    if (wgs >= 512) return 1;
+    long long s = 1024 / (wgs > 0 ? wgs : 1);
+    const long long most = Tk / (n > 0 ? n : 1) / 256;
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+}  // namespace
+
+extern "C" size_t casmtr_packed_attn_ws_floats(long long Tq, long long Tk, int nseq, int H, int Hk, int D) {
+    if (Tq <= 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || D <= 0) return 0;
+    const int s = split_count(Tq, Tk, nseq, H, Hk);
+    return s > 1 ? (size_t)s * Tq * H * (D + 2) : 0;
+}
+
+extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, float* ws, const int* cu_q, const int* cu_k,
+                                      const int* len_k, long long Tq, long long Tk, int nseq, int H, int Hk, int D, long long qts, long long qhs,
+                                      long long kts, long long khs, long long vts, long long vhs, float scale, int causal, int dtype,
+                                      casmtr_stream_t stream) {
+    if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale < INFINITY) ||
+        Tq * (H / Hk) > 0x7fffffffLL || Tk > 0x7fffffffLL || Tq > 0x7fffffffLL)
+        return CASMTR_ERR_UNSUPPORTED;
+    if (Tq == 0) return 0;
+    const int splits = split_count(Tq, Tk, nseq, H, Hk), G = H / Hk;
+    if (splits > 1 && !ws) return CASMTR_ERR_UNSUPPORTED;
+    const long long rows = Tq * H, wgs = slot_count(Tq, G, nseq, 32 * FWD_NW) * Hk;
+    if (wgs > 0x7fffffffLL) return CASMTR_ERR_UNSUPPORTED;
+    AttnArgs a{q, k, v, o, lse, ws, ws ? ws + (long long)splits * rows * D : nullptr, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk},
+               qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits, scale * 1.44269504088896341f};
+    ProfScope ps(CASMTR_PROF_GLUE, (hipStream_t)stream, "packed_attn_kernel");
+    const bool ok = with_type(dtype, [&](auto tv) {
+        typedef decltype(tv) T;
+        const dim3 grid((unsigned)wgs, (unsigned)splits), block(64 * FWD_NW);
+        constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+        if (D <= 32) hipLaunchKernelGGL((packed_attn_kernel<T, 32, 64, FWD_NW>), grid, block, 0, (hipStream_t)stream, a);
+        else if (D <= 64) hipLaunchKernelGGL((packed_attn_kernel<T, 64, 64, FWD_NW>), grid, block, 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL((packed_attn_kernel<T, 128, BN, FWD_NW>), grid, block, 0, (hipStream_t)stream, a);
+        if (splits > 1) hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+    });
+    if (!ok) return CASMTR_ERR_UNSUPPORTED;
+    CASMTR_CHECK_LAUNCH();
+    return 0;
+}

@@ -1,0 +1,227 @@
+// Shared pieces of the packed attention kernels (packed_attn.hip, packed_attn_bwd.hip): matrix fragments, LDS tiles, the map from workgroups
+// to tiles of sequences, visibility.
+//
+// One matrix shape throughout, v_mfma_f32_32x32x16: D[32][32] += A[32][16] B[16][32].  Lane l = 32 h + r holds, as A, row r and as B, column r of
+// the contraction indices 8 h .. 8 h + 7 (eight 16-bit elements, one ds_read_b128); of D it holds column r and the rows 8 (i / 4) + 4 h + i % 4,
+// i = 0..15.  fp32 operands use the same distribution: eight v_mfma_f32_32x32x2_f32, the e-th on element e of every lane.
+// A product's result becomes the next product's B operand without leaving its lanes: the rows of D that a lane holds are contraction
+// indices then, and any order of them will do as long as A is read in the same one.  So scores are computed transposed (keys x rows): a
+// lane owns one query row, its maximum and sum are in-lane but for one exchange between the halves, and the probabilities feed the second
+// product from registers.  The A operand of that product is a tile transposed (head columns x keys), which ds_read_b64_tr_b16 reads from the
+// row-major tile: four consecutive rows of one column per lane and instruction.
+#pragma once
+#include "token_types.hpp"
+
+namespace casmtr {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;   // 16 bytes at any element
+
+template <typename T> struct FragOf { typedef T type __attribute__((ext_vector_type(8))); };
+template <typename T> using frag_t = typename FragOf<T>::type;
+
+__device__ __forceinline__ f32x16 mma(const frag_t<bf16_t>& a, const frag_t<bf16_t>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const frag_t<f16_t>& a, const frag_t<f16_t>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const frag_t<float>& a, const frag_t<float>& b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// An LDS tile of ROWS x DP elements in 16-byte chunks.  Rows are read at one chunk by 32 lanes (ds_read_b128) and, transposed, four rows x four
+// chunks by 32 lanes (16-bit) or two rows x eight chunks by 64 lanes (fp32); the exclusive-or below puts the chunks of each such access on
+// different banks (256 bytes = all 64 banks = one "line" of 16 chunks; rows shorter than that share a line).
+template <typename T, int DP>
+struct Tile {
+    static constexpr int EPC = 16 / (int)sizeof(T);          // elements of a chunk
+    static constexpr int CPR = DP / EPC;                     // chunks of a row
+    static constexpr int RB = DP * (int)sizeof(T);           // bytes of a row
+    static __device__ __forceinline__ int off(int row, int chunk) {
+        if constexpr (CPR >= 16) {
+            const int f = sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 2) & 1) << 3) | ((row & 3) << 1) | ((row >> 3) & 1);
+            return row * RB + ((chunk ^ f) << 4);
+        } else if constexpr (CPR == 8) {
+            const int line = row >> 1;
+            const int f = sizeof(T) == 2 ? ((line & 1) << 2) | ((line >> 1) & 3) : (((line >> 1) & 1) << 3) | (line & 7);
+            return line * 256 + (((((row & 1) << 3) | chunk) ^ f) << 4);
+        } else {
+            const int line = row >> 2;
+            return line * 256 + (((((row & 3) << 2) | chunk) ^ (line & 3)) << 4);
+        }
+    }
+    // A / B operand: row `row` (per lane), contraction indices 16 s + 8 h ..
+    static __device__ __forceinline__ frag_t<T> rows(const char* tile, int row, int s, int h) {
+        frag_t<T> f;
+        if constexpr (sizeof(T) == 2) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(tile + off(row, 2 * s + h));
+            __builtin_memcpy(&f, &v, 16);
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + off(row, 4 * s + 2 * h));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + off(row, 4 * s + 2 * h + 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { f[e] = a[e]; f[4 + e] = b[e]; }
+        }
+        return f;
+    }
+    // transposed A operand: column col0 + r of the tile's rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3} -- the order in which a result's
+    // registers 8 t .. 8 t + 7 hold its rows
+    static __device__ __forceinline__ frag_t<T> cols(const char* tile, int row0, int col0, int lane) {
+        frag_t<T> f;
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            // the 16 lanes of a group name four rows x 16 columns (8 bytes each); lane i receives column i of the four rows
+            const int i = lane & 15, row = row0 + 4 * h + (i >> 2), col = col0 + (lane & 16) + 4 * (i & 3);
+            const int half = (col & 4) << 1;
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + off(row, col >> 3) + half));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + off(row + 8, col >> 3) + half));
+            __builtin_memcpy(&f, &a, 8);
+            __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &b, 8);
+        } else {
+            const int col = col0 + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                f[e] = *reinterpret_cast<const float*>(tile + off(row0 + 8 * (e >> 2) + 4 * h + (e & 3), col >> 2) + (col & 3) * 4);
+        }
+        return f;
+    }
+};
+
+// 16 bytes of a row from column col on; columns from D on are zero
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, int col, int D) {
+    constexpr int EPC = 16 / (int)sizeof(T);
+    if (col + EPC <= D) return *reinterpret_cast<const u32x4_any*>(row + col);
+    T v[EPC];
+#pragma unroll
+    for (int i = 0; i < EPC; ++i) v[i] = col + i < D ? row[col + i] : (T)0.f;
+    u32x4 r;
+    __builtin_memcpy(&r, v, 16);
+    return r;
+}
+// the fragment of a row held in global memory: columns 16 s + 8 h ..
+template <typename T>
+__device__ __forceinline__ frag_t<T> load_frag(const T* row, int s, int h, int D) {
+    frag_t<T> f;
+    const int col = 16 * s + 8 * h;
+    const u32x4 a = load_chunk(row, col, D);
+    __builtin_memcpy(&f, &a, 16);
+    if constexpr (sizeof(T) == 4) {
+        const u32x4 b = load_chunk(row, col + 4, D);
+        __builtin_memcpy(reinterpret_cast<char*>(&f) + 16, &b, 16);
+    }
+    return f;
+}
+
+// registers 8 t .. 8 t + 7 of a result as the next product's operand
+template <typename T>
+__device__ __forceinline__ frag_t<T> to_frag(const f32x16& c, int t) {
+    frag_t<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (T)c[8 * t + e];
+    return f;
+}
+
+__device__ __forceinline__ float max_halves(float v) {   // max / sum with the other half of the wave
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// whether any of the wave's eight elements is infinite or NaN
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(const frag_t<T>& f) {
+    constexpr unsigned EXP = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, bf16_t>::value ? 0x7f807f80u : 0x7c007c00u;
+    constexpr unsigned ONE = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, bf16_t>::value ? 0x00800080u : 0x04000400u;
+    constexpr unsigned TOP = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    unsigned w[sizeof(frag_t<T>) / 4], acc = 0;
+    __builtin_memcpy(w, &f, sizeof(w));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(w) / 4; ++i) acc |= (w[i] & EXP) + ONE;   // an exponent of all ones carries into the sign's place
+    return __any((acc & TOP) != 0);
+}
+// c += A B where some (contraction index, column) pairs are hidden: B is zero there, and what A holds at an index must not reach the columns
+// that it is hidden from, infinities and NaN included (0 * inf is NaN).  If A is finite that is the plain product; otherwise its finite
+// elements are multiplied first and the others follow index by index, a column taking the sum only where it sees the index: every
+// column gets the bits that it would get without them.  sees(n): whether this lane's column sees the index that element n & 7 of
+// half n >> 3 stands for.
+template <typename T, typename Sees>
+__device__ __forceinline__ f32x16 mma_hidden(const frag_t<T>& a, const frag_t<T>& b, f32x16 c, int h, Sees&& sees) {
+    if (__builtin_expect(!any_not_finite<T>(a), 1)) return mma(a, b, c);
+    frag_t<T> fin;
+    unsigned odd = 0;   // this lane's elements that are not finite
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool ok = __builtin_fabsf((float)a[e]) < INFINITY;
+        fin[e] = ok ? a[e] : (T)0.f;
+        odd |= (ok ? 0u : 1u) << (8 * h + e);
+    }
+    c = mma(fin, b, c);
+    for (int n = 0; n < 16; ++n) {
+        if (!__any((odd >> n) & 1u)) continue;
+        frag_t<T> a1, b1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool on = n == 8 * h + e;
+            a1[e] = on && ((odd >> n) & 1u) ? a[e] : (T)0.f;
+            b1[e] = on ? b[e] : (T)0.f;
+        }
+        const f32x16 d = mma(a1, b1, c);
+        if (sees(n)) c = d;
+    }
+    return c;
+}
+
+// ---- sequences
+struct PackedSeqs {
+    const int *cu_q, *cu_k, *len_k;   // cu_q, cu_k [n + 1]; len_k [n] or NULL: keys in use of each sequence's share
+    int n, G;                         // sequences; query heads per key head
+    int causal;
+    long long Tq, Tk;
+};
+struct Span { int begin, count; };
+// the rows of "sequence" s = -1 .. n: -1 and n are the rows before the first and behind the last one, which belong to none.  Whatever the
+// arrays hold, spans stay inside the tensors.
+__device__ __forceinline__ int bound_of(const int* cu, int s, int n, long long T) {
+    if (s < 0) return 0;
+    return s > n ? (int)T : (int)max(0LL, min((long long)cu[s], T));
+}
+__device__ __forceinline__ Span span_of(const int* cu, int s, int n, long long T) {
+    const int b = bound_of(cu, s, n, T);
+    return {b, max(0, bound_of(cu, s + 1, n, T) - b)};
+}
+__device__ __forceinline__ Span keys_of(const PackedSeqs& p, int s) {
+    if (s < 0 || s >= p.n) return {0, 0};
+    Span k = span_of(p.cu_k, s, p.n, p.Tk);
+    if (p.len_k) k.count = max(0, min(k.count, p.len_k[s]));
+    return k;
+}
+// Tiles of SIZE rows (a token counts `per` rows): sequence s owns the slots from bound(s) * per / SIZE + s + 1 on, which leaves it at least
+// as many as it has tiles, whatever the lengths.  So the host sizes the grid from the tensors' shapes alone -- it never waits for the
+// lengths -- and a workgroup finds its tile with a binary search; slots too many leave at once.
+__host__ __device__ __forceinline__ long long slot_count(long long T, int per, int n, int size) { return T * per / size + n + 2; }
+__device__ __forceinline__ int seq_of_slot(const int* cu, int n, long long T, int per, int size, long long slot, int* tile) {
+    int lo = -1, hi = n;   // the last s whose first slot is <= slot
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((long long)bound_of(cu, mid, n, T) * per / size + mid + 1 <= slot) lo = mid;
+        else hi = mid - 1;
+    }
+    *tile = (int)(slot - ((long long)bound_of(cu, lo, n, T) * per / size + lo + 1));
+    return lo;
+}
+}  // namespace casmtr

@@ -911,3 +911,52 @@ def rotary(q, k, positions, inv_freq, layout="half", gain=1.0, inverse=False):
                                                 int(positions.dtype == torch.int64), int(layout == "interleaved"), float(gain), int(bool(inverse)),
                                                 *qs, *ks, _TOKEN_TYPES[q.dtype], _stream()), "rotary_fwd")
     return oq, ok
+
+
+def _packed_args(q, k, v, cu_q, cu_k, len_k, scale):
+    """checks of the packed attention's operands -> (cu_k, scale, sizes, strides)"""
+    qs, ks, vs = _chk_heads(q, "q"), _chk_heads(k, "k", q), _chk_heads(v, "v", q)
+    (Tq, H, D), (Tk, Hk, _) = q.shape, k.shape
+    if k.shape != v.shape or k.shape[2] != D:
+        raise RuntimeError(f"packed_attn: k and v must be [keys, kv_heads, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise RuntimeError(f"packed_attn: {H} query heads do not share {Hk} key heads evenly")
+    if not 1 <= D <= 128:
+        raise RuntimeError(f"packed_attn: head dimension {D} is not in 1..128")
+    if cu_k is None:
+        if Tk != Tq:
+            raise RuntimeError("packed_attn: without cu_k the keys are the rows' own and k must have q's rows")
+        cu_k = cu_q
+    for t, n in ((cu_q, "cu_q"), (cu_k, "cu_k"), (len_k, "len_k")):
+        if t is not None and (_chk(t, n, torch.int32).dim() != 1 or t.device != q.device):
+            raise RuntimeError(f"{n} must be an int32 vector on {q.device}")
+    n = cu_q.numel() - 1
+    if n < 0 or cu_k.numel() != n + 1 or (len_k is not None and len_k.numel() != n):
+        raise RuntimeError("packed_attn: cu_q and cu_k must have one more element than there are sequences, len_k as many")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise RuntimeError(f"packed_attn: scale must be positive and finite, got {scale}")
+    return cu_k, scale, (Tq, Tk, n, H, Hk, D), (*qs, *ks, *vs)
+
+
+def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, want_lse=False):
+    """Softmax attention over packed sequences of different lengths, q [Tq,H,D], k, v [Tk,Hk,D] (fp32 / fp16 / bf16, D <= 128; H % Hk == 0:
+    consecutive groups of H / Hk query heads share a key head; any token and head strides) -> out [Tq,H,D] (, lse fp32 [Tq,H]).
+    Sequence s owns the rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32, on the device; cu_k=None: the same).
+    len_k [sequences]: only the first len_k[s] keys of a share are in use -- a cache: one row per sequence in q (cu_q = 0, 1, 2, ...),
+    cu_k = 0, capacity, 2 capacity, ... and len_k the tokens so far is the form for single tokens; the keys are then split over workgroups.
+    causal: row i sees the keys j <= i + nk - nq.  A row that sees no key, or belongs to no sequence, gives 0 (lse -inf).  What lies behind
+    a sequence's keys is never read into a result, and infinities or NaN in keys and values reach only the rows that see them.
+    Scores, softmax statistics and sums are fp32; probabilities are rounded to the values' type for the product with them.  No host
+    synchronisation; safe to capture into a HIP graph."""
+    cu_k, scale, sizes, strides = _packed_args(q, k, v, cu_q, cu_k, len_k, scale)
+    Tq, Tk, n, H, Hk, D = sizes
+    out = torch.empty((Tq, H, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((Tq, H), device=q.device, dtype=torch.float32) if want_lse else None
+    l = _lib.lib()
+    wsf = l.casmtr_packed_attn_ws_floats(*sizes)
+    ws = torch.empty(wsf, device=q.device, dtype=torch.float32) if wsf else None
+    with torch.cuda.device(q.device):
+        _lib.check(l.casmtr_packed_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(ws), _ptr(cu_q), _ptr(cu_k), _ptr(len_k), *sizes, *strides,
+                                            scale, int(bool(causal)), _TOKEN_TYPES[q.dtype], _stream()), "packed_attn_fwd")
+    return (out, lse) if want_lse else out

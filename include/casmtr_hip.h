@@ -343,6 +343,20 @@ int casmtr_rotary_fwd(const void* q, const void* k, const void* pos, const doubl
                       int npairs, int axes, int pos_is_i64, int layout, float gain, int inverse, long long q_token_stride, long long q_head_stride,
                       long long k_token_stride, long long k_head_stride, int dtype, casmtr_stream_t stream);
 
+/* Attention over packed sequences: q, o [Tq,H,D], k, v [Tk,Hk,D] (H % Hk == 0: consecutive groups of query heads share a key head; D <= 128),
+ * sequence s = rows cu_q[s] .. cu_q[s+1] - 1 of q against rows cu_k[s] .. cu_k[s+1] - 1 of k and v, of which len_k != NULL takes the first
+ * len_k[s] (a cache of fixed shares).  cu_q, cu_k [nseq+1], len_k [nseq] int32 on the device, non-decreasing; they are read by the
+ * kernels alone, which stay inside the tensors whatever they hold.
+ *   o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j),  lse_i = log sum_j exp(scale q_i . k_j)      (lse [Tq,H] fp32 or NULL)
+ * over all keys of the sequence, or, causal, those with j <= i + nk - nq (the last row sees every key).  A row that sees no key, and a
+ * row outside every sequence, gives 0 and -inf.  Infinities and NaN in keys and values reach the rows that see them and no others.
+ * scale > 0.  ws: casmtr_packed_attn_ws_floats() floats (0: none needed).                                                       */
+size_t casmtr_packed_attn_ws_floats(long long Tq, long long Tk, int nseq, int H, int Hk, int D);
+int casmtr_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, float* ws, const int* cu_q, const int* cu_k,
+                           const int* len_k, long long Tq, long long Tk, int nseq, int H, int Hk, int D, long long q_token_stride,
+                           long long q_head_stride, long long k_token_stride, long long k_head_stride, long long v_token_stride,
+                           long long v_head_stride, float scale, int causal, int dtype, casmtr_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------------------------
  * Measurement hooks (no reference counterpart): per-kernel launch durations from HIP events recorded on the
  * launch stream.  Off by default.  casmtr_prof_enable(1) starts a fresh collection; casmtr_prof_read() waits for

@@ -10,7 +10,8 @@ def test_operators_reject_host_tensors():
     x, w = torch.zeros(4, 32), torch.ones(32)
     q = torch.zeros(4, 2, 32)
     for call in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm_quant(x, w), lambda: ops.rms_norm_bwd(x, x, w, torch.ones(4)),
-                 lambda: ops.rotary(q, q, torch.arange(4), torch.ones(8, dtype=torch.float64))):
+                 lambda: ops.rotary(q, q, torch.arange(4), torch.ones(8, dtype=torch.float64)),
+                 lambda: ops.packed_attn(q, q, q, torch.tensor([0, 4], dtype=torch.int32))):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
 
@@ -35,6 +36,13 @@ def test_c_entries_refuse_sizes():
     assert rot(T=0) == 0 and rot(Hq=0, Hk=0) == 0
     assert rot(n=33) == bad and rot(n=0) == bad and rot(axes=3) == bad and rot(axes=2, n=31) == bad and rot(layout=2) == bad and rot(dtype=7) == bad
     assert rot(D=4096, n=1025) == bad and rot(Hq=1 << 20, D=64) == bad and rot(T=-1) == bad
+    attn = lambda Tq=8, Tk=8, n=1, H=4, Hk=2, D=64, scale=0.1, dtype=2, ws=p: l.casmtr_packed_attn_fwd(p, p, p, p, None, ws, p, p, None, Tq, Tk, n, H, Hk, D, H * D, D,
+                                                                                                   Hk * D, D, Hk * D, D, scale, 0, dtype, None)
+    assert attn(Tq=0) == 0
+    assert attn(Tq=-1) == bad and attn(Tk=-1) == bad and attn(n=-1) == bad and attn(H=3) == bad and attn(Hk=0) == bad and attn(D=129) == bad and attn(D=0) == bad
+    assert attn(scale=0.0) == bad and attn(scale=-1.0) == bad and attn(scale=math.nan) == bad and attn(scale=math.inf) == bad and attn(dtype=3) == bad
+    assert attn(Tq=1 << 31) == bad and attn(Tk=1 << 31) == bad
+    assert l.casmtr_packed_attn_ws_floats(1, 1 << 20, 1, 8, 8, 128) > 0 and attn(Tq=1, Tk=1 << 20, ws=None) == bad   # split keys need the workspace
 
 
 def test_rotary_freqs():
