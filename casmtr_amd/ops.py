@@ -960,3 +960,21 @@ def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, 
         _lib.check(l.casmtr_packed_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(ws), _ptr(cu_q), _ptr(cu_k), _ptr(len_k), *sizes, *strides,
                                             scale, int(bool(causal)), _TOKEN_TYPES[q.dtype], _stream()), "packed_attn_fwd")
     return (out, lse) if want_lse else out
+
+
+def packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
+    """Gradient of packed_attn: grad like out (contiguous), out and lse as the forward pass returned them -> (dq, dk, dv), contiguous; dk and dv
+    sum over the heads that share a key head.  No atomics: the same call gives the same bits."""
+    cu_k, scale, sizes, strides = _packed_args(q, k, v, cu_q, cu_k, len_k, scale)
+    Tq, Tk, n, H, Hk, D = sizes
+    for t, name, shape, dtype in ((grad, "grad", (Tq, H, D), q.dtype), (out, "out", (Tq, H, D), q.dtype), (lse, "lse", (Tq, H), torch.float32)):
+        if tuple(_chk(t, name, dtype).shape) != shape or t.device != q.device:
+            raise RuntimeError(f"packed_attn_bwd: {name} must be {shape} on {q.device}")
+    dq = torch.empty((Tq, H, D), device=q.device, dtype=q.dtype)
+    dk, dv = (torch.empty((Tk, Hk, D), device=q.device, dtype=q.dtype) for _ in range(2))
+    delta = torch.empty((Tq, H), device=q.device, dtype=torch.float32)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().casmtr_packed_attn_bwd(_ptr(grad), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(delta),
+                                                     _ptr(cu_q), _ptr(cu_k), _ptr(len_k), *sizes, *strides, scale, int(bool(causal)),
+                                                     _TOKEN_TYPES[q.dtype], _stream()), "packed_attn_bwd")
+    return dq, dk, dv

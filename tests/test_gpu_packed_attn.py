@@ -5,6 +5,10 @@ ds = (D + 8) u scale sum_d |q_d k_d| + 4 u |s|.  A probability is off by 2 ds re
 (half(T); fp32: not at all), and products and sum add up to nk terms in fp32: (nk + 32) u.  So
   |o - ref| <= (half16 + 2 ds + (nk + 32) u) sum_j p_j |v_j| + half(T) |ref| + half a subnormal step,
   |lse - ref| <= ds + (nk + 32) u + 4 u |lse|.
+Backward: p is recomputed from the scores and lse, off by ep = 2 ds + (nk + 32) u + 4 u |lse| + 4 u relative to itself; do . v is off by (D + 8) u sum |do v|;
+delta = do . o by the output's tolerance, sum |do| tol(o), and (D + 8) u sum |do o|.  So ds is off by
+  eds = p (ep |do . v - delta| + (D + 8) u sum |do v| + edelta) + half16 |ds| + half a subnormal step,
+and the products add n terms: (n + 32) u of the summed magnitudes.
 """
 import math
 
@@ -75,6 +79,42 @@ def reference(q, k, v, lens, causal, scale, starts=None):
     return out, tol + half(q.dtype) * out.abs() + sub(q.dtype), lse, ltol
 
 
+def reference_grads(g, q, k, v, lens, causal, scale, otol):
+    """-> (dq, tol), (dk, tol), (dv, tol)"""
+    H, Hk, D = q.shape[1], k.shape[1], q.shape[2]
+    z = lambda t: torch.zeros(t.shape, dtype=torch.float64, device="cuda")
+    dq, dk, dv, tq, tk, tv = z(q), z(k), z(v), z(q), z(k), z(v)
+    r, low = step16(q.dtype), (0.0 if q.dtype == torch.float32 else sub(q.dtype))
+    q0 = k0 = 0
+    for a, b in lens:
+        if a and b:
+            vis = seen(a, b, causal)
+            any_ = vis.any(1, keepdim=True)
+            for h in range(H):
+                m = h // (H // Hk)
+                qq, gg, kk, vv = q[q0:q0 + a, h].double(), g[q0:q0 + a, h].double(), k[k0:k0 + b, m].double(), v[k0:k0 + b, m].double()
+                sc = (qq @ kk.t() * scale).masked_fill(~vis, -math.inf)
+                err = ((D + 8) * U * scale * (qq.abs() @ kk.abs().t()) + 4 * U * sc.abs()).masked_fill(~vis, 0).amax(1, keepdim=True)
+                lse = torch.logsumexp(sc, 1, keepdim=True).masked_fill(~any_, 0)
+                p = torch.softmax(sc, 1).masked_fill(~any_, 0)
+                o, dp = p @ vv, gg @ vv.t()
+                ds = p * (dp - (gg * o).sum(1, keepdim=True))
+                ep = 2 * err + (b + 36) * U + 4 * U * lse.abs()
+                edelta = (gg.abs() * (otol[q0:q0 + a, h] + (D + 8) * U * o.abs())).sum(1, keepdim=True)
+                eds = (p * (ep * (dp - (gg * o).sum(1, keepdim=True)).abs() + (D + 8) * U * (gg.abs() @ vv.abs().t()) + edelta) + r * ds.abs() + low) * vis
+                epp = (p * (ep + r) + low) * vis
+                dq[q0:q0 + a, h] = ds @ kk * scale
+                tq[q0:q0 + a, h] = scale * ((eds + (b + 32) * U * ds.abs()) @ kk.abs())
+                n = a * (H // Hk) + 32
+                dk[k0:k0 + b, m] += ds.t() @ qq * scale
+                tk[k0:k0 + b, m] += scale * ((eds + n * U * ds.abs()).t() @ qq.abs())
+                dv[k0:k0 + b, m] += p.t() @ gg
+                tv[k0:k0 + b, m] += (epp + n * U * p).t() @ gg.abs()
+        q0, k0 = q0 + a, k0 + b
+    fin = lambda x, t: (x, t + half(q.dtype) * x.abs() + sub(q.dtype))
+    return fin(dq, tq), fin(dk, tk), fin(dv, tv)
+
+
 def check(got, lse, ref):
     out, tol, rl, ltol = ref
     assert ((got.double() - out).abs() <= tol).all()
@@ -95,6 +135,91 @@ def test_forward(name, H, Hk, D, dt):
             out, lse = ops.packed_attn(q, k, v, cq, ck, causal=causal, scale=scale, want_lse=True)
             check(out, lse, reference(q, k, v, lens, causal, scale or D ** -0.5))
             assert torch.equal(ops.packed_attn(q, k, v, cq, ck, causal=causal, scale=scale), out)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("H,Hk,D", HEADS)
+@pytest.mark.parametrize("name", list(LENS))
+def test_backward(name, H, Hk, D, dt):
+    from casmtr_amd import ops
+    lens = LENS[name]
+    q, k, v, cq, ck = make(lens, H, Hk, D, dt, seed=1)
+    g = torch.randn(q.shape, generator=torch.Generator().manual_seed(2)).to(dt).cuda()
+    for causal in (False, True):
+        out, lse = ops.packed_attn(q, k, v, cq, ck, causal=causal, want_lse=True)
+        got = ops.packed_attn_bwd(g, q, k, v, out, lse, cq, ck, causal=causal)
+        otol = reference(q, k, v, lens, causal, D ** -0.5)[1]
+        for x, (ref, tol) in zip(got, reference_grads(g, q, k, v, lens, causal, D ** -0.5, otol)):
+            assert x.dtype == dt and ((x.double() - ref).abs() <= tol).all()
+        again = ops.packed_attn_bwd(g, q, k, v, out, lse, cq, ck, causal=causal)
+        assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+def test_backward_cache_and_views():
+    """shares that are not in use get zero gradients whatever they hold; operands are views, the gradient of a sum is a broadcast view"""
+    from casmtr_amd import ops
+    from casmtr_amd.functions.packed_attention import packed_attention_op
+    used, cap, rows = [40, 0, 7, 64], 64, 5
+    q, k, v, cq, _ = make([(rows, cap)] * 4, 4, 2, 32, torch.float32, tail=0)
+    ck, ln = cu([cap] * 4), torch.tensor(used, dtype=torch.int32).cuda()
+    packed = torch.cat([torch.arange(s * cap, s * cap + n) for s, n in enumerate(used)]).cuda()
+    want = [t.clone().requires_grad_() for t in (q, k[packed], v[packed])]
+    packed_attention_op(*want, cq, cu(used), None, True).sum().backward()
+    for s, n in enumerate(used):
+        k[s * cap + n:(s + 1) * cap], v[s * cap + n:(s + 1) * cap] = math.nan, math.inf
+    hm = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1).requires_grad_()
+    got = [hm(q), hm(k), hm(v)]
+    packed_attention_op(*got, cq, ck, ln, True).sum().backward()
+    assert torch.equal(got[0].grad, want[0].grad)
+    rest = torch.ones(4 * cap, dtype=torch.bool, device="cuda")
+    rest[packed] = False
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a.grad[packed], b.grad) and (a.grad[rest] == 0).all()
+
+
+def test_gradient_against_differences():
+    """central differences of sum(g o) in 64 bits along random directions; the kernel's gradients are held to the formula's tolerances"""
+    from casmtr_amd.functions.packed_attention import packed_attention_op
+    lens = [(30, 44), (17, 17)]
+    q, k, v, cq, ck = make(lens, 4, 2, 24, torch.float32, tail=0)
+    g = torch.randn_like(q)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention_op(*leaves, cq, ck, None, True, 0.25), leaves, g)
+    dirs = [torch.randn_like(t).double() for t in leaves]
+
+    def loss(e):
+        x = [t.detach().double() + e * d for t, d in zip(leaves, dirs)]
+        return (g.double() * reference(*x, lens, True, 0.25)[0]).sum()
+
+    diff = (loss(1e-4) - loss(-1e-4)) / 2e-4      # the third derivative's share is 1e-8 of the scale
+    got = sum((a.double() * d).sum() for a, d in zip(grads, dirs))
+    mag = sum((a.double() * d).abs().sum() for a, d in zip(grads, dirs))
+    assert abs(got - diff) <= 1e-5 * mag
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (3, 1, 128), (2, 2, 32)])
+def test_hidden_infinities_backward(H, Hk, D, dt):
+    """a key's infinities stay away from the gradients of rows that do not see it, a row's from those of keys that it does not see"""
+    from casmtr_amd import ops
+    lens = [(150, 150), (90, 90)]
+    q, k, v, cq, ck = make(lens, H, Hk, D, dt)
+    g = torch.randn(q.shape, device="cuda").to(dt)
+
+    def grads(q, k, v, g):
+        out, lse = ops.packed_attn(q, k, v, cq, ck, causal=True, want_lse=True)
+        return ops.packed_attn_bwd(g, q, k, v, out, lse, cq, ck, causal=True)
+
+    clean = grads(q, k, v, g)
+    for bad in (math.nan, math.inf):
+        k2, v2 = k.clone(), v.clone()
+        k2[100, :, 3], v2[100, :, 5] = bad, bad
+        dq, _, _ = grads(q, k2, v2, g)
+        assert torch.equal(dq[:100], clean[0][:100]) and torch.equal(dq[150:], clean[0][150:])
+        q2, g2 = q.clone(), g.clone()
+        q2[60, :, 3], g2[60, :, 5] = bad, bad
+        _, dk, dv = grads(q2, k, v, g2)
+        assert torch.equal(dk[61:], clean[1][61:]) and torch.equal(dv[61:], clean[2][61:])
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -211,5 +336,11 @@ def test_refusals():
                 lambda: ops.packed_attn(q.double(), k.double(), v.double(), cq), lambda: ops.packed_attn(q[..., ::2], k[..., ::2], v[..., ::2], cq),
                 lambda: ops.packed_attn(q, k[..., :32], v[..., :32], cq), lambda: ops.packed_attn(*(torch.zeros(9, 2, 136, device="cuda"),) * 3, cq),
                 lambda: ops.packed_attn(q[0], k[0], v[0], cq), lambda: ops.packed_attn(q, k[:, :0], v[:, :0], cq), lambda: ops.packed_attn(q, k, v, cq.view(1, 2))):
+        with pytest.raises(RuntimeError):
+            bad()
+    out, lse = ops.packed_attn(q, k, v, cq, want_lse=True)
+    for bad in (lambda: ops.packed_attn_bwd(out[:8], q, k, v, out, lse, cq), lambda: ops.packed_attn_bwd(out.float(), q, k, v, out, lse, cq),
+                lambda: ops.packed_attn_bwd(out, q, k, v, out, lse[:, :2], cq), lambda: ops.packed_attn_bwd(out, q, k, v, out, lse.half(), cq),
+                lambda: ops.packed_attn_bwd(out[:1].expand(9, 4, 64), q, k, v, out, lse, cq), lambda: ops.packed_attn_bwd(out, q, k, v, out.cpu(), lse, cq)):
         with pytest.raises(RuntimeError):
             bad()

@@ -43,6 +43,10 @@ def test_c_entries_refuse_sizes():
     assert attn(scale=0.0) == bad and attn(scale=-1.0) == bad and attn(scale=math.nan) == bad and attn(scale=math.inf) == bad and attn(dtype=3) == bad
     assert attn(Tq=1 << 31) == bad and attn(Tk=1 << 31) == bad
     assert l.casmtr_packed_attn_ws_floats(1, 1 << 20, 1, 8, 8, 128) > 0 and attn(Tq=1, Tk=1 << 20, ws=None) == bad   # split keys need the workspace
+    bwd = lambda Tq=8, Tk=8, n=1, H=4, Hk=2, D=64, scale=0.1, dtype=2: l.casmtr_packed_attn_bwd(*(p,) * 12, None, Tq, Tk, n, H, Hk, D, H * D, D, Hk * D, D, Hk * D, D,
+                                                                                        scale, 0, dtype, None)
+    assert bwd(Tq=0, Tk=0) == 0
+    assert bwd(Tq=-1) == bad and bwd(Tk=-1) == bad and bwd(n=-1) == bad and bwd(H=3) == bad and bwd(D=129) == bad and bwd(scale=0.0) == bad and bwd(dtype=3) == bad
 
 
 def test_rotary_freqs():
