@@ -5,7 +5,7 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax.  A tile's rows are (token, head of the group) pairs, token-major, so
 // all G heads of a key head use one copy of its keys, and a single token of G heads is one tile.  A workgroup has four waves of 32 rows; K and V
-// tiles of BN keys go through LDS, the next tile's loads in flight while this one is multiplied.
+// tiles of BN keys go through LDS in two stages: the next tile's loads are in flight while this one is multiplied, one barrier per tile.
 #include "packed_attn.hpp"
 
 using namespace casmtr;
@@ -25,14 +25,14 @@ struct AttnArgs {
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a maximum grew by more than 8 bits: exp2 stays below 256, far from any overflow
 
-template <typename T, int DP, int BN, int NW>
-__global__ __launch_bounds__(64 * NW) void packed_attn_kernel(const AttnArgs a) {
+template <typename T, int DP, int BN, int NW, bool DMA>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
     typedef Tile<T, DP> L;
     constexpr int BM = 32 * NW, NT = 64 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
     constexpr int NCH = BN * L::CPR / NT;           // chunks per thread of a K (V) tile
     constexpr int TB = BN * L::RB;                  // bytes of a tile
     __shared__ __attribute__((aligned(256))) char smem[4 * TB];   // K, V of two stages
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, r = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int hk = blockIdx.x % a.Hk, G = a.s.G;
     int tile;
     const int seq = seq_of_slot(a.s.cu_q, a.s.n, a.s.Tq, G, BM, (long long)(gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk), &tile);   // later rows see more keys: first
@@ -59,95 +59,123 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_kernel(const AttnArgs a) 
         for (int s = 0; s < KS; ++s) qf[s] = load_frag(qr, s, h, a.D);
     }
     f32x16 acc[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = zero16();
-    float m = -INFINITY, l = 0.f;
+    float m, l;
 
     const T* kb = (const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs;
     const T* vb = (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs;
-    u32x4 kr[NCH], vr[NCH];
-    const auto fetch = [&](int t) {
+    // K and V tiles: straight into LDS, or (rows that are not 16-byte aligned) through registers
+    TileDma<T, DP, BN, NW> kd, vd;
+    u32x4 kr[DMA ? 1 : NCH], vr[DMA ? 1 : NCH];
+    const unsigned lds0 = lds_byte_addr(smem);
+    if constexpr (DMA) { kd.init(tid, a.kts, a.D); vd.init(tid, a.vts, a.D); }
+    const auto fetch = [&](int t, int stage) {
+        if constexpr (DMA) {
+            kd.issue(kb + (long long)t * BN * a.kts, keys.count - t * BN, lds0 + 2 * stage * TB, wave);
+            vd.issue(vb + (long long)t * BN * a.vts, keys.count - t * BN, lds0 + (2 * stage + 1) * TB, wave);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int id = tid + NT * i, rr = t * BN + id / L::CPR, c = (id % L::CPR) * L::EPC;
-            kr[i] = u32x4{0, 0, 0, 0};
-            vr[i] = u32x4{0, 0, 0, 0};
-            if (rr < keys.count && c < a.D) {
-                kr[i] = load_chunk(kb + (long long)rr * a.kts, c, a.D);
-                vr[i] = load_chunk(vb + (long long)rr * a.vts, c, a.D);
+            for (int i = 0; i < NCH; ++i) {
+                const int id = tid + NT * i, rr = t * BN + id / L::CPR, c = (id % L::CPR) * L::EPC;
+                kr[i] = u32x4{0, 0, 0, 0};
+                vr[i] = u32x4{0, 0, 0, 0};
+                if (rr < keys.count && c < a.D) {
+                    kr[i] = load_chunk(kb + (long long)rr * a.kts, c, a.D);
+                    vr[i] = load_chunk(vb + (long long)rr * a.vts, c, a.D);
+                }
             }
         }
     };
     const auto put = [&](int stage) {
+        if constexpr (!DMA) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
-            *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = kr[i];
-            *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = vr[i];
+            for (int i = 0; i < NCH; ++i) {
+                const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
+                *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = kr[i];
+                *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = vr[i];
+            }
         }
     };
-    if (t0 < t1) { fetch(t0); put(0); }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int stage = (t - t0) & 1;
-        if (t + 1 < t1) fetch(t + 1);
-        const char *ks = smem + 2 * stage * TB, *vs = ks + TB;
-        if (t * BN < wave_end) {
-            f32x16 s[NB];
+    // One pass over the keys.  GUARD: with the product that keeps what a row does not see away from it (mma_hidden)
+    const auto pass = [&](auto guard) {
+        constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                s[b] = zero16();
+        for (int d = 0; d < DB; ++d) acc[d] = zero16();
+        m = -INFINITY;
+        l = 0.f;
+        if (t0 < t1) { fetch(t0, 0); put(0); }
+        for (int t = t0; t < t1; ++t) {
+            const int stage = (t - t0) & 1;
+            if constexpr (DMA) glds_wait<0>();
+            __syncthreads();   // this tile is in LDS; nobody reads the other stage any more
+            if (t + 1 < t1) fetch(t + 1, stage ^ 1);
+            const char *ks = smem + 2 * stage * TB, *vs = ks + TB;
+            if (t * BN < wave_end) {
+                f32x16 s[NB];
 #pragma unroll
-                for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, 32 * b + r, st, h), qf[st], s[b]);
-            }
-            const bool hidden = (t + 1) * BN > wave_all;
-            if (hidden) {
+                for (int b = 0; b < NB; ++b) {
+                    s[b] = zero16();
+#pragma unroll
+                    for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, 32 * b + r, st, h), qf[st], s[b]);
+                }
+                const bool hidden = (t + 1) * BN > wave_all;
+                if (hidden) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[b][i] = -INFINITY;
+                }
+                float mx = s[0][0];
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[b][i] = -INFINITY;
-            }
-            float mx = s[0][0];
+                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+                mx = max_halves(mx) * a.scale;
+                const bool up = mx > m + RESCALE_AT;   // (also the first tile: m = -inf); per row, so that a row's bits do not depend on its neighbours
+                if (__any(up)) {
+                    const float f = !up ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+                    m = up ? mx : m;
+                    l *= f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+                    for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-            mx = max_halves(mx) * a.scale;
-            const bool up = mx > m + RESCALE_AT;   // (also the first tile: m = -inf); per row, so that a row's bits do not depend on its neighbours
-            if (__any(up)) {
-                const float f = !up ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-                m = up ? mx : m;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[d][i] *= f;
-            }
-            const float mm = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.scale, -mm));
-                    l += s[b][i];
+                        for (int i = 0; i < 16; ++i) acc[d][i] *= f;
                 }
+                const float mm = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const frag_t<T> p = to_frag<T>(s[b], tt);   // probabilities below 256 rounded to the values' type; l sums the unrounded ones
-                    const int k0 = 32 * b + 16 * tt;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const frag_t<T> vt = L::cols(vs, k0, 32 * d, lane);
-                        if (!hidden) acc[d] = mma(vt, p, acc[d]);
-                        else acc[d] = mma_hidden<T>(vt, p, acc[d], h, [&](int n) { return t * BN + k0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3) < limit; });
+                    for (int i = 0; i < 16; ++i) {
+                        s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.scale, -mm));
+                        l += s[b][i];
                     }
-                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) {
+                        const frag_t<T> p = to_frag<T>(s[b], tt);   // probabilities below 256 rounded to the values' type; l sums the unrounded ones
+                        const int k0 = 32 * b + 16 * tt;
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            const frag_t<T> vt = L::cols(vs, k0, 32 * d, lane);
+                            if constexpr (!GUARD) acc[d] = mma(vt, p, acc[d]);
+                            else acc[d] = mma_hidden<T>(vt, p, acc[d], h, [&](int n) { return t * BN + k0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3) < limit; });
+                        }
+                    }
+            }
+            if (t + 1 < t1) put(stage ^ 1);
         }
-        if (t + 1 < t1) put(stage ^ 1);
-        __syncthreads();
+    };
+    pass(std::false_type{});
+    // Hidden keys are weighted with exact zeros, so an infinity or NaN among hidden values is the only way by which one can reach a row that
+    // does not see it -- and then the row's sum is not finite.  Rare enough to do it again, carefully, when that is seen.
+    if (a.s.causal) {
+        float worst = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) worst += __builtin_fabsf(acc[d][i]);
+        if (__syncthreads_or(!(worst < INFINITY))) pass(std::true_type{});
     }
     l = add_halves(l);
     if (row >= nrow) return;
@@ -252,10 +280,17 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
     const bool ok = with_type(dtype, [&](auto tv) {
         typedef decltype(tv) T;
         const dim3 grid((unsigned)wgs, (unsigned)splits), block(64 * FWD_NW);
-        constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-        if (D <= 32) hipLaunchKernelGGL((packed_attn_kernel<T, 32, 64, FWD_NW>), grid, block, 0, (hipStream_t)stream, a);
-        else if (D <= 64) hipLaunchKernelGGL((packed_attn_kernel<T, 64, 64, FWD_NW>), grid, block, 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL((packed_attn_kernel<T, 128, BN, FWD_NW>), grid, block, 0, (hipStream_t)stream, a);
+        constexpr int BN = sizeof(T) == 2 ? 64 : 32;   // the widest heads' tiles: 64 KB of LDS either way
+        const bool dma = TileDma<T, 128, 64, FWD_NW>::fits(k, kts, khs, D) && TileDma<T, 128, 64, FWD_NW>::fits(v, vts, vhs, D);
+#define FWD_LAUNCH(DP, BN)                                                                                                    \
+    do {                                                                                                                      \
+        if (dma) hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, FWD_NW, true>), grid, block, 0, (hipStream_t)stream, a);   \
+        else hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, FWD_NW, false>), grid, block, 0, (hipStream_t)stream, a);      \
+    } while (0)
+        if (D <= 32) FWD_LAUNCH(32, 64);
+        else if (D <= 64) FWD_LAUNCH(64, 64);
+        else FWD_LAUNCH(128, BN);
+#undef FWD_LAUNCH
         if (splits > 1) hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
     });
     if (!ok) return CASMTR_ERR_UNSUPPORTED;

@@ -60,6 +60,21 @@ struct Tile {
             return line * 256 + (((((row & 3) << 2) | chunk) ^ (line & 3)) << 4);
         }
     }
+    // the (row, chunk) that lies at 16-byte slot p of the tile
+    static __device__ __forceinline__ void at(int p, int& row, int& chunk) {
+        if constexpr (CPR >= 16) {
+            row = p / CPR;
+            chunk = (off(row, p % CPR) - row * RB) >> 4;   // (the exclusive-or is its own inverse)
+        } else if constexpr (CPR == 8) {
+            const int line = p >> 4, x = ((off(2 * line, 0) - line * 256) >> 4) ^ (p & 15);
+            row = 2 * line + (x >> 3);
+            chunk = x & 7;
+        } else {
+            const int line = p >> 4, x = (line & 3) ^ (p & 15);
+            row = 4 * line + (x >> 2);
+            chunk = x & 3;
+        }
+    }
     // A / B operand: row `row` (per lane), contraction indices 16 s + 8 h ..
     static __device__ __forceinline__ frag_t<T> rows(const char* tile, int row, int s, int h) {
         frag_t<T> f;
@@ -123,6 +138,45 @@ __device__ __forceinline__ frag_t<T> load_frag(const T* row, int s, int h, int D
     }
     return f;
 }
+
+// ---- a tile straight from global memory into LDS (buffer_load_dwordx4 ... lds: 64 lanes x 16 bytes to consecutive LDS addresses, no
+// registers; the layout's exclusive-or is applied to the SOURCE addresses).  The buffer's size is set per tile to the rows that are left, and
+// what lies behind it -- rows past the sequence's keys, columns past D -- arrives as zero.  Needs 16-byte aligned rows of whole chunks that do not
+// overlap.  Inline asm, so that the compiler does not drain the loads in flight before every LDS read: the kernels wait with glds_wait().
+template <typename T, int DP, int ROWS, int NW>
+struct TileDma {
+    typedef Tile<T, DP> L;
+    static constexpr int N = ROWS * L::CPR / (64 * NW);   // instructions per wave
+    unsigned voff[N];
+    unsigned row_bytes, width;
+    __device__ __forceinline__ void init(int tid, long long stride, int D) {
+        row_bytes = (unsigned)(stride * (long long)sizeof(T));
+        width = (unsigned)(D * (int)sizeof(T));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            int row, chunk;
+            L::at(tid + 64 * NW * i, row, chunk);
+            voff[i] = chunk * L::EPC < D ? (unsigned)row * row_bytes + (unsigned)chunk * 16u : 0x80000000u;
+        }
+    }
+    // rows_left >= 1 rows from `base` on; lds: the tile's LDS byte address
+    __device__ __forceinline__ void issue(const T* base, int rows_left, unsigned lds, int wave) const {
+        const unsigned long long b = (unsigned long long)base;
+        const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(b >> 32)),
+                            (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(min(rows_left, ROWS) - 1) * row_bytes + width)), 0x00020000u};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (unsigned)(64 * NW * i + 64 * wave) * 16u));
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff[i]), "s"(dst), "s"(rsrc) : "memory");
+        }
+    }
+    // whether rows of this stride can be read so
+    static __host__ __forceinline__ bool fits(const void* p, long long token_stride, long long head_stride, int D) {
+        const long long e = (long long)sizeof(T);
+        return D * e % 16 == 0 && (unsigned long long)p % 16 == 0 && token_stride * e % 16 == 0 && head_stride * e % 16 == 0 && token_stride >= D &&
+               token_stride * e * (ROWS + 1) < 0x7fffffffLL;
+    }
+};
 
 // registers 8 t .. 8 t + 7 of a result as the next product's operand
 template <typename T>
