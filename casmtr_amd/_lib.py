@@ -69,6 +69,7 @@ SIGNATURES = {
     "casmtr_rotary_fwd": (_I, [_P] * 6 + [_LL] + [_I] * 7 + [_F, _I] + [_LL] * 4 + [_I, _P]),
     "casmtr_packed_attn_ws_floats": (_SZ, [_LL, _LL, _I, _I, _I, _I]),
     "casmtr_packed_attn_fwd": (_I, [_P] * 9 + [_LL, _LL] + [_I] * 4 + [_LL] * 6 + [_F, _I, _I, _P]),
+    "casmtr_packed_attn_bwd_ws_floats": (_SZ, [_LL, _LL, _I, _I, _I, _I]),
     "casmtr_packed_attn_bwd": (_I, [_P] * 13 + [_LL, _LL] + [_I] * 4 + [_LL] * 6 + [_F, _I, _I, _P]),
     "casmtr_prof_enable": (None, [_I]),
     "casmtr_debug_set": (None, [_I]),

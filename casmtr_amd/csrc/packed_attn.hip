@@ -28,10 +28,8 @@ constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a m
 template <typename T, int DP, int BN, int NW, bool DMA>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
     typedef Tile<T, DP> L;
-    constexpr int BM = 32 * NW, NT = 64 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
-    constexpr int NCH = BN * L::CPR / NT;           // chunks per thread of a K (V) tile
-    constexpr int TB = BN * L::RB;                  // bytes of a tile
-    __shared__ __attribute__((aligned(256))) char smem[4 * TB];   // K, V of two stages
+    constexpr int BM = 32 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
+    __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BN, NW, DMA>::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int hk = blockIdx.x % a.Hk, G = a.s.G;
     int tile;
@@ -61,40 +59,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
     f32x16 acc[DB];
     float m, l;
 
-    const T* kb = (const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs;
-    const T* vb = (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs;
-    // K and V tiles: straight into LDS, or (rows that are not 16-byte aligned) through registers
-    TileDma<T, DP, BN, NW> kd, vd;
-    u32x4 kr[DMA ? 1 : NCH], vr[DMA ? 1 : NCH];
-    const unsigned lds0 = lds_byte_addr(smem);
-    if constexpr (DMA) { kd.init(tid, a.kts, a.D); vd.init(tid, a.vts, a.D); }
-    const auto fetch = [&](int t, int stage) {
-        if constexpr (DMA) {
-            kd.issue(kb + (long long)t * BN * a.kts, keys.count - t * BN, lds0 + 2 * stage * TB, wave);
-            vd.issue(vb + (long long)t * BN * a.vts, keys.count - t * BN, lds0 + (2 * stage + 1) * TB, wave);
-        } else {
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int id = tid + NT * i, rr = t * BN + id / L::CPR, c = (id % L::CPR) * L::EPC;
-                kr[i] = u32x4{0, 0, 0, 0};
-                vr[i] = u32x4{0, 0, 0, 0};
-                if (rr < keys.count && c < a.D) {
-                    kr[i] = load_chunk(kb + (long long)rr * a.kts, c, a.D);
-                    vr[i] = load_chunk(vb + (long long)rr * a.vts, c, a.D);
-                }
-            }
-        }
-    };
-    const auto put = [&](int stage) {
-        if constexpr (!DMA) {
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
-                *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = kr[i];
-                *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = vr[i];
-            }
-        }
-    };
+    TilePair<T, DP, BN, NW, DMA> kv;
+    kv.init(smem, tid, wave, a.kts, a.vts, a.D);
+    kv.of((const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
     // One pass over the keys.  GUARD: with the product that keeps what a row does not see away from it (mma_hidden)
     const auto pass = [&](auto guard) {
         constexpr bool GUARD = decltype(guard)::value;
@@ -102,13 +69,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         m = -INFINITY;
         l = 0.f;
-        if (t0 < t1) { fetch(t0, 0); put(0); }
+        if (t0 < t1) kv.fetch(t0, 0);
         for (int t = t0; t < t1; ++t) {
             const int stage = (t - t0) & 1;
-            if constexpr (DMA) glds_wait<0>();
+            kv.arrived(stage);
             __syncthreads();   // this tile is in LDS; nobody reads the other stage any more
-            if (t + 1 < t1) fetch(t + 1, stage ^ 1);
-            const char *ks = smem + 2 * stage * TB, *vs = ks + TB;
+            if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
+            const char *ks = kv.first(stage), *vs = kv.second(stage);
             if (t * BN < wave_end) {
                 f32x16 s[NB];
 #pragma unroll
@@ -163,7 +130,6 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
                         }
                     }
             }
-            if (t + 1 < t1) put(stage ^ 1);
         }
     };
     pass(std::false_type{});

@@ -178,6 +178,58 @@ struct TileDma {
     }
 };
 
+// Two tiles of ROWS x DP in two stages of LDS (K and V, or q and the output's gradient): rows t ROWS .. of `a` and `b`, zero from `count` rows and D
+// columns on.  fetch(t, stage) starts tile t, arrived(stage) is called by every thread before the barrier that precedes its use.
+// DMA: straight into LDS; otherwise (rows that are not 16-byte aligned) through registers, written when the tile is due.
+template <typename T, int DP, int ROWS, int NW, bool DMA>
+struct TilePair {
+    typedef Tile<T, DP> L;
+    static constexpr int NT = 64 * NW, NCH = ROWS * L::CPR / NT, TB = ROWS * L::RB, BYTES = 4 * TB;
+    static_assert(ROWS * L::CPR % NT == 0, "whole chunks per thread");
+    char* smem;
+    const T *a, *b;
+    long long as, bs;
+    int count, D, tid, wave;
+    TileDma<T, DP, ROWS, NW> ad, bd;
+    u32x4 ar[DMA ? 1 : NCH], br[DMA ? 1 : NCH];
+    __device__ __forceinline__ void init(char* smem_, int tid_, int wave_, long long as_, long long bs_, int D_) {
+        smem = smem_; tid = tid_; wave = wave_; as = as_; bs = bs_; D = D_;
+        if constexpr (DMA) { ad.init(tid, as, D); bd.init(tid, bs, D); }
+    }
+    __device__ __forceinline__ void of(const T* a_, const T* b_, int count_) { a = a_; b = b_; count = count_; }
+    __device__ __forceinline__ const char* first(int stage) const { return smem + 2 * stage * TB; }
+    __device__ __forceinline__ const char* second(int stage) const { return smem + (2 * stage + 1) * TB; }
+    __device__ __forceinline__ void fetch(int t, int stage) {
+        if constexpr (DMA) {
+            const unsigned lds = lds_byte_addr(smem) + 2 * stage * TB;
+            ad.issue(a + (long long)t * ROWS * as, count - t * ROWS, lds, wave);
+            bd.issue(b + (long long)t * ROWS * bs, count - t * ROWS, lds + TB, wave);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int id = tid + NT * i, rr = t * ROWS + id / L::CPR, c = (id % L::CPR) * L::EPC;
+                ar[i] = u32x4{0, 0, 0, 0};
+                br[i] = u32x4{0, 0, 0, 0};
+                if (rr < count && c < D) {
+                    ar[i] = load_chunk(a + (long long)rr * as, c, D);
+                    br[i] = load_chunk(b + (long long)rr * bs, c, D);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void arrived(int stage) {
+        if constexpr (DMA) glds_wait<0>();
+        else {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
+                *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = ar[i];
+                *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = br[i];
+            }
+        }
+    }
+};
+
 // registers 8 t .. 8 t + 7 of a result as the next product's operand
 template <typename T>
 __device__ __forceinline__ frag_t<T> to_frag(const f32x16& c, int t) {

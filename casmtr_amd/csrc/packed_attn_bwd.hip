@@ -1,8 +1,8 @@
 // Attention over packed sequences, backward.  With p_ij = exp(scale q_i . k_j - lse_i):
 //   delta_i = sum_d do_i o_i;  ds_ij = p_ij (do_i . v_j - delta_i) scale
 //   dq_i = sum_j ds_ij k_j;    dk_j = sum_i ds_ij q_i;    dv_j = sum_i p_ij do_i
-// Two kernels, no atomics: one owns query rows and walks the keys (dq, and delta on the way), one owns keys and walks the query rows of all
-// heads that share them (dk, dv: the sum over the group is in the accumulator).  The scores are computed twice for it -- 7 products
+// No atomics: one kernel owns query rows and walks the keys (dq, and delta on the way), one owns keys and walks the query rows of all
+// heads that share them (dk, dv: the sum over the group is in the accumulator; in parts that a third kernel adds where there are few keys).  The scores are computed twice for it -- 7 products
 // instead of 5 -- and results repeat bit for bit.
 #include "packed_attn.hpp"
 
@@ -13,10 +13,11 @@ struct BwdArgs {
     const void *q, *k, *v, *o, *g;     // o, g (the gradient of o): [Tq, H, D] contiguous
     const float* lse;
     float* delta;                      // [Tq, H]
+    float* part;                       // splits > 1: [splits][dk, dv][Tk * Hk * D] partial sums
     void *dq, *dk, *dv;                // contiguous
     PackedSeqs s;
     long long qts, qhs, kts, khs, vts, vhs;
-    int H, Hk, D;
+    int H, Hk, D, splits;
     float scale, scale_log2;
 };
 constexpr float LOG2E = 1.44269504088896341f;
@@ -41,14 +42,23 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], int h
         }
 }
 
+template <int DB>
+__device__ __forceinline__ bool not_finite(const f32x16 (&acc)[DB]) {
+    float worst = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) worst += __builtin_fabsf(acc[d][i]);
+    return !(worst < INFINITY);
+}
+
 // dq: a workgroup's rows are (token, head) pairs as in the forward kernel
-template <typename T, int DP, int BN, int NW>
-__global__ __launch_bounds__(64 * NW) void packed_attn_dq_kernel(const BwdArgs a) {
+template <typename T, int DP, int BN, int NW, bool DMA>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_kernel(const BwdArgs a) {
     typedef Tile<T, DP> L;
-    constexpr int BM = 32 * NW, NT = 64 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
-    constexpr int NCH = BN * L::CPR / NT, TB = BN * L::RB;
-    __shared__ __attribute__((aligned(256))) char smem[4 * TB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, r = lane & 31;
+    constexpr int BM = 32 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
+    __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BN, NW, DMA>::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int hk = blockIdx.x % a.Hk, G = a.s.G;
     int tile;
     const int seq = seq_of_slot(a.s.cu_q, a.s.n, a.s.Tq, G, BM, (long long)(gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk), &tile);
@@ -81,39 +91,21 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dq_kernel(const BwdArgs a
     const float lse = a.lse[out_row], lse2 = lse == -INFINITY ? 0.f : lse * LOG2E;   // (a row that sees nothing: every key is hidden below)
     if (h == 0 && row < nrow) a.delta[out_row] = delta;
     f32x16 acc[DB];
+    TilePair<T, DP, BN, NW, DMA> kv;
+    kv.init(smem, tid, wave, a.kts, a.vts, a.D);
+    kv.of((const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
+    const auto pass = [&](auto guard) {
+        constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = zero16();
-
-    const T* kb = (const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs;
-    const T* vb = (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs;
-    u32x4 kr[NCH], vr[NCH];
-    const auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int id = tid + NT * i, rr = t * BN + id / L::CPR, c = (id % L::CPR) * L::EPC;
-            kr[i] = u32x4{0, 0, 0, 0};
-            vr[i] = u32x4{0, 0, 0, 0};
-            if (rr < keys.count && c < a.D) {
-                kr[i] = load_chunk(kb + (long long)rr * a.kts, c, a.D);
-                vr[i] = load_chunk(vb + (long long)rr * a.vts, c, a.D);
-            }
-        }
-    };
-    const auto put = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
-            *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = kr[i];
-            *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = vr[i];
-        }
-    };
-    if (0 < t1) { fetch(0); put(0); }
-    __syncthreads();
-    for (int t = 0; t < t1; ++t) {
-        const int stage = t & 1;
-        if (t + 1 < t1) fetch(t + 1);
-        const char *ks = smem + 2 * stage * TB, *vs = ks + TB;
-        if (t * BN < wave_end) {
+        for (int d = 0; d < DB; ++d) acc[d] = zero16();
+        if (0 < t1) kv.fetch(0, 0);
+        for (int t = 0; t < t1; ++t) {
+            const int stage = t & 1;
+            kv.arrived(stage);
+            __syncthreads();
+            if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
+            const char *ks = kv.first(stage), *vs = kv.second(stage);
+            if (t * BN >= wave_end) continue;
             const bool hidden = (t + 1) * BN > wave_all;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -127,7 +119,11 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dq_kernel(const BwdArgs a
                 for (int i = 0; i < 16; ++i) {
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, -lse2));
                     s[i] = p * (dp[i] - delta);
-                    if (hidden && t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[i] = 0.f;
+                }
+                if (hidden) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[i] = 0.f;
                 }
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
@@ -136,44 +132,42 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dq_kernel(const BwdArgs a
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
                         const frag_t<T> kt = L::cols(ks, k0, 32 * d, lane);
-                        if (!hidden) acc[d] = mma(kt, ds, acc[d]);
+                        if constexpr (!GUARD) acc[d] = mma(kt, ds, acc[d]);
                         else acc[d] = mma_hidden<T>(kt, ds, acc[d], h, [&](int n) { return t * BN + k0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3) < limit; });
                     }
                 }
             }
         }
-        if (t + 1 < t1) put(stage ^ 1);
-        __syncthreads();
+    };
+    pass(std::false_type{});
+    if (a.s.causal) {   // as in the forward kernel: a sum that is not finite may have met a hidden infinity
+        if (__syncthreads_or(not_finite(acc))) pass(std::true_type{});
     }
     if (row < nrow) store_row<T, DB>((T*)a.dq + out_row * a.D, acc, h, a.D, a.scale);
 }
 
-// dk, dv: a workgroup owns BN = 32 NW keys of one key head, a wave 32 of them (K and V stay in its registers), and walks the (token, head)
-// rows of the group in tiles of BM
-template <typename T, int DP, int BM, int NW>
-__global__ __launch_bounds__(64 * NW) void packed_attn_dkv_kernel(const BwdArgs a) {
+// dk, dv: a workgroup owns BN = 32 NW keys of one key head, a wave 32 of them (K and V stay in its registers), and walks the rows of the heads that
+// share it, head by head in tiles of BM tokens
+template <typename T, int DP, int BM, int NW, bool DMA>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void packed_attn_dkv_kernel(const BwdArgs a) {
     typedef Tile<T, DP> L;
-    constexpr int BN = 32 * NW, NT = 64 * NW, KS = DP / 16, MB = BM / 32, DB = DP / 32;
-    constexpr int NCH = BM * L::CPR / NT, TB = BM * L::RB;
-    static_assert(BM <= NT, "a thread stages one row's statistics");
-    __shared__ __attribute__((aligned(256))) char smem[4 * TB];          // q, g of two stages
+    constexpr int BN = 32 * NW, KS = DP / 16, MB = BM / 32, DB = DP / 32;
+    static_assert(BM <= 64 * NW, "a thread stages one row's statistics");
+    __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BM, NW, DMA>::BYTES];
     __shared__ __attribute__((aligned(16))) float stat[2][2][BM];        // lse (in bits), delta of two stages
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, r = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int hk = blockIdx.x % a.Hk, G = a.s.G;
     int tile;
     const int seq = seq_of_slot(a.s.cu_k, a.s.n, a.s.Tk, 1, BN, (long long)(blockIdx.x / a.Hk), &tile);   // earlier keys are seen by more rows: first
     const Span share = span_of(a.s.cu_k, seq, a.s.n, a.s.Tk), keys = keys_of(a.s, seq);
     const Span rows = seq >= 0 && seq < a.s.n ? span_of(a.s.cu_q, seq, a.s.n, a.s.Tq) : Span{0, 0};
     if ((long long)tile * BN >= share.count) return;
-    const int key0 = tile * BN, key = key0 + 32 * wave + r;      // keys of the share that are not in use get zero gradients
-    const int shift = keys.count - rows.count, nrow = rows.count * G;
+    const int key0 = tile * BN, wk = key0 + 32 * wave, key = wk + r;      // keys of the share that are not in use get zero gradients
+    const int shift = keys.count - rows.count;
     const bool used = key < keys.count;
-    const int first = !used ? 0x7fffffff : a.s.causal ? max(0, key - shift) : 0;   // this lane's key is seen by the tokens [first, count)
-    // tokens that see some key of the workgroup / the wave, tokens that see all of the wave's keys
-    const int wg_first = key0 >= keys.count ? rows.count : a.s.causal ? min(rows.count, max(0, key0 - shift)) : 0;
-    const int wk = key0 + 32 * wave;
-    const int wave_first = wk >= keys.count ? rows.count : a.s.causal ? min(rows.count, max(0, wk - shift)) : 0;
-    const int wave_all = wk + 32 > keys.count ? 0x7fffffff : a.s.causal ? max(0, wk + 31 - shift) : 0;
+    // a key is seen by the tokens from first_of(key) on: of the lane's key, of the first of the wave and of the workgroup, of the wave's last
+    const auto first_of = [&](int j) { return j >= keys.count ? rows.count : a.s.causal ? min(rows.count, max(0, j - shift)) : 0; };
+    const int first = first_of(key), wg_first = first_of(key0), wave_first = first_of(wk), wave_all = first_of(wk + 31);
     const int kc = max(0, min(key, keys.count - 1));
     frag_t<T> kf[KS], vf[KS];
     {
@@ -186,52 +180,45 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dkv_kernel(const BwdArgs 
         }
     }
     f32x16 dk[DB], dv[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
-
-    const int t0 = (int)((long long)wg_first * G / BM), t1 = (nrow + BM - 1) / BM;
-    u32x4 qr[NCH], gr[NCH];
+    const int t0 = wg_first / BM, per = (rows.count + BM - 1) / BM - t0;   // tiles of a head
+    int n0 = 0, turns = wg_first < rows.count ? per * G : 0;                // of all heads, of this split
+    if (a.splits > 1) {
+        const int each = (turns + a.splits - 1) / a.splits;
+        n0 = min(turns, each * (int)blockIdx.y);
+        turns = min(turns, n0 + each);
+    }
+    TilePair<T, DP, BM, NW, DMA> qg;
+    qg.init(smem, tid, wave, a.qts, (long long)a.H * a.D, a.D);
     float sl = 0.f, sd = 0.f;
-    const auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int id = tid + NT * i, rr = t * BM + id / L::CPR, c = (id % L::CPR) * L::EPC;
-            qr[i] = u32x4{0, 0, 0, 0};
-            gr[i] = u32x4{0, 0, 0, 0};
-            if (rr < nrow && c < a.D) {
-                const int tok = rr / G, head = hk * G + rr % G;
-                qr[i] = load_chunk((const T*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs, c, a.D);
-                gr[i] = load_chunk((const T*)a.g + ((long long)(rows.begin + tok) * a.H + head) * a.D, c, a.D);
-            }
-        }
+    const auto fetch = [&](int n, int stage) {   // turn n: tile t0 + n % per of the group's head n / per
+        const int hd = hk * G + n / per, t = t0 + n % per;
         if (tid < BM) {
-            const int rr = t * BM + tid;
+            const int tok = t * BM + tid;
             sl = sd = 0.f;
-            if (rr < nrow) {
-                const long long at = (long long)(rows.begin + rr / G) * a.H + hk * G + rr % G;
+            if (tok < rows.count) {
+                const long long at = (long long)(rows.begin + tok) * a.H + hd;
                 const float x = a.lse[at];
                 sl = x == -INFINITY ? 0.f : x * LOG2E;
                 sd = a.delta[at];
             }
         }
+        qg.of((const T*)a.q + (long long)rows.begin * a.qts + hd * a.qhs, (const T*)a.g + ((long long)rows.begin * a.H + hd) * a.D, rows.count);
+        qg.fetch(t, stage);
     };
-    const auto put = [&](int stage) {
+    const auto pass = [&](auto guard) {
+        constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int id = tid + NT * i, o = L::off(id / L::CPR, id % L::CPR);
-            *reinterpret_cast<u32x4*>(smem + 2 * stage * TB + o) = qr[i];
-            *reinterpret_cast<u32x4*>(smem + (2 * stage + 1) * TB + o) = gr[i];
-        }
-        if (tid < BM) { stat[stage][0][tid] = sl; stat[stage][1][tid] = sd; }
-    };
-    if (t0 < t1) { fetch(t0); put(0); }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int stage = (t - t0) & 1;
-        if (t + 1 < t1) fetch(t + 1);
-        const char *qs = smem + 2 * stage * TB, *gs = qs + TB;
-        if (min((t + 1) * BM - 1, nrow - 1) / G >= wave_first && wave_first < rows.count) {
-            const bool hidden = t * BM / G < wave_all || (t + 1) * BM > nrow;
+        for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+        if (n0 < turns) fetch(n0, 0);
+        for (int n = n0; n < turns; ++n) {
+            const int stage = (n - n0) & 1, t = t0 + n % per;
+            if (tid < BM) { stat[stage][0][tid] = sl; stat[stage][1][tid] = sd; }
+            qg.arrived(stage);
+            __syncthreads();
+            if (n + 1 < turns) fetch(n + 1, stage ^ 1);
+            const char *qs = qg.first(stage), *gs = qg.second(stage);
+            if ((t + 1) * BM <= wave_first) continue;
+            const bool hidden = t * BM < wave_all || (t + 1) * BM > rows.count;
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
                 f32x16 s = zero16(), dp = zero16();
@@ -240,15 +227,6 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dkv_kernel(const BwdArgs 
                     s = mma(L::rows(qs, 32 * b + r, st, h), kf[st], s);
                     dp = mma(L::rows(gs, 32 * b + r, st, h), vf[st], dp);
                 }
-                unsigned vis = 0xffffu;   // registers whose row sees this lane's key
-                if (hidden) {
-                    vis = 0;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int rr = t * BM + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                        vis |= (rr < nrow && rr / G >= first ? 1u : 0u) << i;
-                    }
-                }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const f32x4 l4 = *reinterpret_cast<const f32x4*>(&stat[stage][0][32 * b + 8 * g + 4 * h]);
@@ -256,37 +234,46 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dkv_kernel(const BwdArgs 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = 4 * g + e;
-                        const bool on = (vis >> i) & 1u;
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, -l4[e]));
-                        s[i] = on ? p : 0.f;
-                        dp[i] = on ? p * (dp[i] - d4[e]) : 0.f;
+                        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, -l4[e]));
+                        dp[i] = s[i] * (dp[i] - d4[e]);
+                    }
+                }
+                // element n & 7 of half n >> 3 of step tt stands for token t BM + 32 b + 16 tt + 8 (n >> 2 & 1) + 4 (n >> 3) + (n & 3)
+                const int tok0 = t * BM + 32 * b;
+                if (hidden) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int tok = tok0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                        if (tok < first || tok >= rows.count) { s[i] = 0.f; dp[i] = 0.f; }
                     }
                 }
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
                     const frag_t<T> pf = to_frag<T>(s, tt), df = to_frag<T>(dp, tt);   // rounded to the rows' type for the products with them
                     const int r0 = 32 * b + 16 * tt;
-                    // element n & 7 of half n >> 3 stands for row r0 + 8 (n >> 2 & 1) + 4 (n >> 3) + (n & 3)
-                    const auto sees = [&](int n) {
-                        const int rr = t * BM + r0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3);
-                        return rr < nrow && rr / G >= first;
+                    const auto sees = [&](int m) {
+                        const int tok = tok0 + 16 * tt + 8 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3);
+                        return tok >= first && tok < rows.count;
                     };
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        const frag_t<T> gt = L::cols(gs, r0, 32 * d, lane), qt = L::cols(qs, r0, 32 * d, lane);
-                        if (!hidden) {
-                            dv[d] = mma(gt, pf, dv[d]);
-                            dk[d] = mma(qt, df, dk[d]);
-                        } else {
-                            dv[d] = mma_hidden<T>(gt, pf, dv[d], h, sees);
-                            dk[d] = mma_hidden<T>(qt, df, dk[d], h, sees);
-                        }
+                        const frag_t<T> gt = L::cols(gs, r0, 32 * d, lane);
+                        if constexpr (!GUARD) dv[d] = mma(gt, pf, dv[d]);
+                        else dv[d] = mma_hidden<T>(gt, pf, dv[d], h, sees);
+                    }
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const frag_t<T> qt = L::cols(qs, r0, 32 * d, lane);
+                        if constexpr (!GUARD) dk[d] = mma(qt, df, dk[d]);
+                        else dk[d] = mma_hidden<T>(qt, df, dk[d], h, sees);
                     }
                 }
             }
         }
-        if (t + 1 < t1) put(stage ^ 1);
-        __syncthreads();
+    };
+    pass(std::false_type{});
+    if (a.s.causal) {
+        if (__syncthreads_or(not_finite(dk) || not_finite(dv))) pass(std::true_type{});
     }
     if (key >= share.count) return;
     const long long out_row = (long long)(share.begin + key) * a.Hk + hk;
@@ -294,15 +281,53 @@ __global__ __launch_bounds__(64 * NW) void packed_attn_dkv_kernel(const BwdArgs 
 #pragma unroll
         for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     }
+    if (a.splits > 1) {
+        const long long n = a.s.Tk * a.Hk * a.D;
+        float* part = a.part + 2 * n * blockIdx.y + out_row * a.D;
+        store_row<float, DB>(part, dk, h, a.D, a.scale);
+        store_row<float, DB>(part + n, dv, h, a.D, 1.f);
+        return;
+    }
     store_row<T, DB>((T*)a.dk + out_row * a.D, dk, h, a.D, a.scale);
     store_row<T, DB>((T*)a.dv + out_row * a.D, dv, h, a.D, 1.f);
 }
 
+// dk and dv as the sums of their splits, in order
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(const BwdArgs a) {
+    const long long n = a.s.Tk * a.Hk * a.D, i = 8 * ((long long)blockIdx.x * 256 + threadIdx.x);
+    if (i >= n) return;
+    const int m = (int)min(8LL, n - i);
+    const float* part = a.part + (blockIdx.y ? n : 0) + i;
+    float v[8], x[8];
+    load_n(part, v, m);
+    for (int s = 1; s < a.splits; ++s) {
+        load_n(part + 2 * n * s, x, m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+    store_n((T*)(blockIdx.y ? a.dv : a.dk) + i, v, m);
+}
+
 constexpr int BWD_NW = 4;
+
+// Parts that the rows of a key tile are split into.  A key tile walks all rows of all the heads that share it, so few key heads leave the chip to
+// a few long workgroups (6 packed documents up to 4096, 4 key heads, 356 workgroups: 597 us with one part).  Each part costs a write
+// and a read of dk and dv in fp32.
+int split_rows(long long Tk, int n, int Hk) {
+    const long long wgs = slot_count(Tk, 1, n, 32 * BWD_NW) * Hk;
+    return wgs >= 1024 ? 1 : (int)(wgs >= 256 ? 1 + 1023 / wgs : 4);
+}
 }  // namespace
 
+extern "C" size_t casmtr_packed_attn_bwd_ws_floats(long long Tq, long long Tk, int nseq, int H, int Hk, int D) {
+    if (Tq <= 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || D <= 0) return 0;
+    const int s = split_rows(Tk, nseq, Hk);
+    return (size_t)Tq * H + (s > 1 ? (size_t)2 * s * Tk * Hk * D + 3 : 0);
+}
+
 extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk,
-                                      void* dv, float* delta, const int* cu_q, const int* cu_k, const int* len_k, long long Tq, long long Tk, int nseq,
+                                      void* dv, float* ws, const int* cu_q, const int* cu_k, const int* len_k, long long Tq, long long Tk, int nseq,
                                       int H, int Hk, int D, long long qts, long long qhs, long long kts, long long khs, long long vts, long long vhs,
                                       float scale, int causal, int dtype, casmtr_stream_t stream) {
     if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale < INFINITY) ||
@@ -312,22 +337,36 @@ extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* 
     const int G = H / Hk;
     const long long qwgs = slot_count(Tq, G, nseq, 32 * BWD_NW) * Hk, kwgs = slot_count(Tk, 1, nseq, 32 * BWD_NW) * Hk;
     if (qwgs > 0x7fffffffLL || kwgs > 0x7fffffffLL) return CASMTR_ERR_UNSUPPORTED;
-    BwdArgs a{q, k, v, o, g, lse, delta, dq, dk, dv, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk}, qts, qhs, kts, khs, vts, vhs, H, Hk, D, scale,
-              scale * LOG2E};
+    if (Tq > 0 && !ws) return CASMTR_ERR_UNSUPPORTED;
+    const int splits = Tq > 0 ? split_rows(Tk, nseq, Hk) : 1;
+    float* part = ws ? ws + (((size_t)Tq * H + 3) & ~(size_t)3) : nullptr;
+    BwdArgs a{q, k, v, o, g, lse, ws, part, dq, dk, dv, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk}, qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits,
+              scale, scale * LOG2E};
     ProfScope ps(CASMTR_PROF_GLUE, (hipStream_t)stream, "packed_attn_dq_kernel, packed_attn_dkv_kernel");
     with_type(dtype, [&](auto tv) {
         typedef decltype(tv) T;
-        const dim3 block(64 * BWD_NW);
+        const dim3 block(64 * BWD_NW), kgrid((unsigned)kwgs, (unsigned)splits);
+        const hipStream_t st = (hipStream_t)stream;
         constexpr int W = sizeof(T) == 2 ? 64 : 32;   // the widest head's tiles: 64 KB of LDS either way
-#define BWD_LAUNCH(DP, TILE, RTILE)                                                                                                                     \
-    do {                                                                                                                                         \
-        if (Tq > 0) hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, TILE, BWD_NW>), dim3((unsigned)qwgs), block, 0, (hipStream_t)stream, a);    \
-        if (Tk > 0) hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, RTILE, BWD_NW>), dim3((unsigned)kwgs), block, 0, (hipStream_t)stream, a);     \
+        typedef TileDma<T, 128, 64, BWD_NW> Dma;
+        const bool kdma = Dma::fits(k, kts, khs, D) && Dma::fits(v, vts, vhs, D), qdma = Dma::fits(q, qts, qhs, D) && Dma::fits(g, (long long)H * D, D, D);
+#define BWD_LAUNCH(DP, TILE, RTILE)                                                                                                    \
+    do {                                                                                                                               \
+        if (Tq > 0) {                                                                                                                  \
+            if (kdma) hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, TILE, BWD_NW, true>), dim3((unsigned)qwgs), block, 0, st, a);   \
+            else hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, TILE, BWD_NW, false>), dim3((unsigned)qwgs), block, 0, st, a);       \
+        }                                                                                                                              \
+        if (Tk > 0) {                                                                                                                  \
+            if (qdma) hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, RTILE, BWD_NW, true>), kgrid, block, 0, st, a); \
+            else hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, RTILE, BWD_NW, false>), kgrid, block, 0, st, a);     \
+        }                                                                                                                              \
     } while (0)
         if (D <= 32) BWD_LAUNCH(32, 64, 64);
         else if (D <= 64) BWD_LAUNCH(64, 64, 32);
         else BWD_LAUNCH(128, W, 32);
 #undef BWD_LAUNCH
+        if (splits > 1 && Tk > 0)
+            hipLaunchKernelGGL((packed_attn_dkv_join_kernel<T>), dim3((unsigned)((Tk * Hk * D + 2047) / 2048), 2), dim3(256), 0, st, a);
     });
     CASMTR_CHECK_LAUNCH();
     return 0;

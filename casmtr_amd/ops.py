@@ -972,9 +972,11 @@ def packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k=None, len_k=None, causal
             raise RuntimeError(f"packed_attn_bwd: {name} must be {shape} on {q.device}")
     dq = torch.empty((Tq, H, D), device=q.device, dtype=q.dtype)
     dk, dv = (torch.empty((Tk, Hk, D), device=q.device, dtype=q.dtype) for _ in range(2))
-    delta = torch.empty((Tq, H), device=q.device, dtype=torch.float32)
+    l = _lib.lib()
+    wsf = l.casmtr_packed_attn_bwd_ws_floats(*sizes)
+    ws = torch.empty(wsf, device=q.device, dtype=torch.float32) if wsf else None
     with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().casmtr_packed_attn_bwd(_ptr(grad), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(delta),
-                                                     _ptr(cu_q), _ptr(cu_k), _ptr(len_k), *sizes, *strides, scale, int(bool(causal)),
-                                                     _TOKEN_TYPES[q.dtype], _stream()), "packed_attn_bwd")
+        _lib.check(l.casmtr_packed_attn_bwd(_ptr(grad), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), _ptr(cu_q),
+                                            _ptr(cu_k), _ptr(len_k), *sizes, *strides, scale, int(bool(causal)), _TOKEN_TYPES[q.dtype], _stream()),
+                   "packed_attn_bwd")
     return dq, dk, dv

@@ -358,9 +358,10 @@ int casmtr_packed_attn_fwd(const void* q, const void* k, const void* v, void* o,
                            long long v_head_stride, float scale, int causal, int dtype, casmtr_stream_t stream);
 /* Its gradient: g [Tq,H,D] the gradient of o (g, o contiguous), lse as written by the forward pass -> dq [Tq,H,D], dk, dv [Tk,Hk,D] (contiguous; zero
  * where a row sees nothing, a key is seen by no row or not in use).  dk and dv sum over the heads that share a key head; all sums have a
- * fixed order.  delta [Tq,H]: workspace.                                                                                          */
+ * fixed order.  ws: casmtr_packed_attn_bwd_ws_floats() floats.                                                                     */
+size_t casmtr_packed_attn_bwd_ws_floats(long long Tq, long long Tk, int nseq, int H, int Hk, int D);
 int casmtr_packed_attn_bwd(const void* g, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk, void* dv,
-                           float* delta, const int* cu_q, const int* cu_k, const int* len_k, long long Tq, long long Tk, int nseq, int H, int Hk, int D,
+                           float* ws, const int* cu_q, const int* cu_k, const int* len_k, long long Tq, long long Tk, int nseq, int H, int Hk, int D,
                            long long q_token_stride, long long q_head_stride, long long k_token_stride, long long k_head_stride,
                            long long v_token_stride, long long v_head_stride, float scale, int causal, int dtype, casmtr_stream_t stream);
 
