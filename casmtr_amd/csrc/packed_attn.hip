@@ -70,13 +70,15 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
         m = -INFINITY;
         l = 0.f;
         if (t0 < t1) kv.fetch(t0, 0);
-        for (int t = t0; t < t1; ++t) {
-            const int stage = (t - t0) & 1;
+        const auto step = [&](int t, auto stage_) {
+            constexpr int stage = decltype(stage_)::value;   // a constant: it goes into the offsets of the LDS reads
             kv.arrived(stage);
             __syncthreads();   // this tile is in LDS; nobody reads the other stage any more
             if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
-            const char *ks = kv.first(stage), *vs = kv.second(stage);
-            if (t * BN < wave_end) {
+            if (t * BN >= wave_end) return;
+            const bool hidden = (t + 1) * BN > wave_all;   // some pair of the tile is hidden
+            {
+                const char *ks = kv.first(stage), *vs = kv.second(stage);
                 f32x16 s[NB];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -84,13 +86,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
 #pragma unroll
                     for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, 32 * b + r, st, h), qf[st], s[b]);
                 }
-                const bool hidden = (t + 1) * BN > wave_all;
                 if (hidden) {
+                    const int lim = limit - t * BN - 4 * h;
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if (t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[b][i] = -INFINITY;
+                            if (32 * b + 8 * (i >> 2) + (i & 3) >= lim) s[b][i] = -INFINITY;
                 }
                 float mx = s[0][0];
 #pragma unroll
@@ -130,6 +132,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
                         }
                     }
             }
+        };
+        for (int t = t0; t < t1; t += 2) {
+            step(t, std::integral_constant<int, 0>{});
+            if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
         }
     };
     pass(std::false_type{});

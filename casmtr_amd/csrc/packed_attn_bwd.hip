@@ -99,14 +99,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         if (0 < t1) kv.fetch(0, 0);
-        for (int t = 0; t < t1; ++t) {
-            const int stage = t & 1;
+        const auto step = [&](int t, auto stage_) {
+            constexpr int stage = decltype(stage_)::value;
             kv.arrived(stage);
             __syncthreads();
             if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
-            const char *ks = kv.first(stage), *vs = kv.second(stage);
-            if (t * BN >= wave_end) continue;
+            if (t * BN >= wave_end) return;
             const bool hidden = (t + 1) * BN > wave_all;
+            const char *ks = kv.first(stage), *vs = kv.second(stage);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 f32x16 s = zero16(), dp = zero16();
@@ -121,9 +121,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
                     s[i] = p * (dp[i] - delta);
                 }
                 if (hidden) {
+                    const int lim = limit - t * BN - 4 * h;
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (t * BN + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= limit) s[i] = 0.f;
+                        if (32 * b + 8 * (i >> 2) + (i & 3) >= lim) s[i] = 0.f;
                 }
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
@@ -137,6 +138,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
                     }
                 }
             }
+        };
+        for (int t = 0; t < t1; t += 2) {
+            step(t, std::integral_constant<int, 0>{});
+            if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
         }
     };
     pass(std::false_type{});
@@ -210,15 +215,16 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
 #pragma unroll
         for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
         if (n0 < turns) fetch(n0, 0);
-        for (int n = n0; n < turns; ++n) {
-            const int stage = (n - n0) & 1, t = t0 + n % per;
+        const auto step = [&](int n, auto stage_) {
+            constexpr int stage = decltype(stage_)::value;
+            const int t = t0 + n % per;
             if (tid < BM) { stat[stage][0][tid] = sl; stat[stage][1][tid] = sd; }
             qg.arrived(stage);
             __syncthreads();
             if (n + 1 < turns) fetch(n + 1, stage ^ 1);
-            const char *qs = qg.first(stage), *gs = qg.second(stage);
-            if ((t + 1) * BM <= wave_first) continue;
+            if ((t + 1) * BM <= wave_first) return;
             const bool hidden = t * BM < wave_all || (t + 1) * BM > rows.count;
+            const char *qs = qg.first(stage), *gs = qg.second(stage);
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
                 f32x16 s = zero16(), dp = zero16();
@@ -241,10 +247,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
                 // element n & 7 of half n >> 3 of step tt stands for token t BM + 32 b + 16 tt + 8 (n >> 2 & 1) + 4 (n >> 3) + (n & 3)
                 const int tok0 = t * BM + 32 * b;
                 if (hidden) {
+                    const int lo = first - tok0 - 4 * h, hi = rows.count - tok0 - 4 * h;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int tok = tok0 + 8 * (i >> 2) + 4 * h + (i & 3);
-                        if (tok < first || tok >= rows.count) { s[i] = 0.f; dp[i] = 0.f; }
+                        const int x = 8 * (i >> 2) + (i & 3);
+                        if (x < lo || x >= hi) { s[i] = 0.f; dp[i] = 0.f; }
                     }
                 }
 #pragma unroll
@@ -269,6 +276,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
                     }
                 }
             }
+        };
+        for (int n = n0; n < turns; n += 2) {
+            step(n, std::integral_constant<int, 0>{});
+            if (n + 1 < turns) step(n + 1, std::integral_constant<int, 1>{});
         }
     };
     pass(std::false_type{});
@@ -316,7 +327,7 @@ constexpr int BWD_NW = 4;
 // and a read of dk and dv in fp32.
 int split_rows(long long Tk, int n, int Hk) {
     const long long wgs = slot_count(Tk, 1, n, 32 * BWD_NW) * Hk;
-    return wgs >= 1024 ? 1 : (int)(wgs >= 256 ? 1 + 1023 / wgs : 4);
+    return wgs >= 2048 ? 1 : (int)(wgs >= 256 ? 1 + 2047 / wgs : 8);
 }
 }  // namespace
 
@@ -362,7 +373,7 @@ extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* 
         }                                                                                                                              \
     } while (0)
         if (D <= 32) BWD_LAUNCH(32, 64, 64);
-        else if (D <= 64) BWD_LAUNCH(64, 64, 32);
+        else if (D <= 64) BWD_LAUNCH(64, 64, W);
         else BWD_LAUNCH(128, W, 32);
 #undef BWD_LAUNCH
         if (splits > 1 && Tk > 0)
