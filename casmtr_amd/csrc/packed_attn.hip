@@ -25,10 +25,13 @@ struct AttnArgs {
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a maximum grew by more than 8 bits: exp2 stays below 256, far from any overflow
 
-template <typename T, int DP, int BN, int NW, bool DMA>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
+// FEW (few rows, long keys): a workgroup has 32 rows, its waves take 32 keys each of a tile and are joined in LDS at the end.  With 128 rows per
+// workgroup a tile takes each wave the whole way through 64 keys, for nothing where three of four waves have no rows of their own.
+template <typename T, int DP, int BN, int NW, bool DMA, bool FEW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
     typedef Tile<T, DP> L;
-    constexpr int BM = 32 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
+    static_assert(!FEW || BN == 32 * NW, "one block of keys per wave");
+    constexpr int BM = FEW ? 32 : 32 * NW, KS = DP / 16, NB = FEW ? 1 : BN / 32, DB = DP / 32;
     __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BN, NW, DMA>::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int hk = blockIdx.x % a.Hk, G = a.s.G;
@@ -38,18 +41,23 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
     const int nrow = rows.count * G;
     if ((long long)tile * BM >= nrow) return;   // a slot too many
     const int row0 = tile * BM;
-    const int row = row0 + 32 * wave + r, rc = min(row, nrow - 1), tok = rc / G, head = hk * G + rc % G;
+    const int wrow = FEW ? 0 : 32 * wave, wkey = FEW ? 32 * wave : 0;   // the wave's rows of the workgroup's, keys of a tile's
+    const int row = row0 + wrow + r, rc = min(row, nrow - 1), tok = rc / G, head = hk * G + rc % G;
     const int shift = keys.count - rows.count;
     const int limit = a.s.causal ? max(0, min(keys.count, tok + shift + 1)) : keys.count;   // this lane's row sees the keys [0, limit)
     // keys that some row of the workgroup / of the wave sees (rows see more the later they are), keys that all rows of the wave see
     const auto limit_at = [&](int rr) { return a.s.causal ? max(0, min(keys.count, min(rr, nrow - 1) / G + shift + 1)) : keys.count; };
-    const int wg_end = limit_at(row0 + BM - 1), wave_end = limit_at(row0 + 32 * wave + 31), wave_all = limit_at(row0 + 32 * wave);
+    const int wg_end = limit_at(row0 + BM - 1), wave_end = limit_at(row0 + wrow + 31), wave_all = limit_at(row0 + wrow);
     int t0 = 0, t1 = (wg_end + BN - 1) / BN;
     if (a.splits > 1) {
         const int per = (t1 + a.splits - 1) / a.splits;
         t0 = min(t1, per * (int)blockIdx.y);
         t1 = min(t1, t0 + per);
     }
+    TilePair<T, DP, BN, NW, DMA> kv;
+    kv.init(smem, tid, wave, a.kts, a.vts, a.D);
+    kv.of((const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
+    if (t0 < t1) kv.fetch(t0, 0);
     frag_t<T> qf[KS];
     {
         const T* qr = (const T*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
@@ -58,10 +66,6 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
     }
     f32x16 acc[DB];
     float m, l;
-
-    TilePair<T, DP, BN, NW, DMA> kv;
-    kv.init(smem, tid, wave, a.kts, a.vts, a.D);
-    kv.of((const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
     // One pass over the keys.  GUARD: with the product that keeps what a row does not see away from it (mma_hidden)
     const auto pass = [&](auto guard) {
         constexpr bool GUARD = decltype(guard)::value;
@@ -69,14 +73,15 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         m = -INFINITY;
         l = 0.f;
-        if (t0 < t1) kv.fetch(t0, 0);
+        if (GUARD && t0 < t1) kv.fetch(t0, 0);   // (the first pass's first tile is under way)
         const auto step = [&](int t, auto stage_) {
             constexpr int stage = decltype(stage_)::value;   // a constant: it goes into the offsets of the LDS reads
             kv.arrived(stage);
             __syncthreads();   // this tile is in LDS; nobody reads the other stage any more
             if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
-            if (t * BN >= wave_end) return;
-            const bool hidden = (t + 1) * BN > wave_all;   // some pair of the tile is hidden
+            const int key0 = t * BN + wkey;
+            if (key0 >= wave_end) return;
+            const bool hidden = key0 + 32 * NB > wave_all;   // some pair of the wave's is hidden
             {
                 const char *ks = kv.first(stage), *vs = kv.second(stage);
                 f32x16 s[NB];
@@ -84,10 +89,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
                 for (int b = 0; b < NB; ++b) {
                     s[b] = zero16();
 #pragma unroll
-                    for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, 32 * b + r, st, h), qf[st], s[b]);
+                    for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, wkey + 32 * b + r, st, h), qf[st], s[b]);
                 }
                 if (hidden) {
-                    const int lim = limit - t * BN - 4 * h;
+                    const int lim = limit - key0 - 4 * h;
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -126,9 +131,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
                         const int k0 = 32 * b + 16 * tt;
 #pragma unroll
                         for (int d = 0; d < DB; ++d) {
-                            const frag_t<T> vt = L::cols(vs, k0, 32 * d, lane);
+                            const frag_t<T> vt = L::cols(vs, wkey + k0, 32 * d, lane);
                             if constexpr (!GUARD) acc[d] = mma(vt, p, acc[d]);
-                            else acc[d] = mma_hidden<T>(vt, p, acc[d], h, [&](int n) { return t * BN + k0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3) < limit; });
+                            else acc[d] = mma_hidden<T>(vt, p, acc[d], h, [&](int n) { return key0 + k0 + 8 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3) < limit; });
                         }
                     }
             }
@@ -150,6 +155,61 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
         if (__syncthreads_or(!(worst < INFINITY))) pass(std::true_type{});
     }
     l = add_halves(l);
+    if constexpr (FEW) {
+        // join the waves: a row's maximum over them, every wave's share times 2^(m - maximum), the shares added in order
+        constexpr int LD = DP + 4;
+        static_assert((NW * 32 * LD + 2 * NW * 32) * 4 <= TilePair<T, DP, BN, NW, DMA>::BYTES, "the shares fit the tiles' LDS");
+        float *share = reinterpret_cast<float*>(smem), *stat = share + NW * 32 * LD;
+        __syncthreads();
+        if (h == 0) { stat[wave * 32 + r] = m; stat[(NW + wave) * 32 + r] = l; }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(share + (wave * 32 + r) * LD + 32 * d + 8 * g + 4 * h) =
+                    f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        __syncthreads();
+        constexpr int CT = DP / 4;   // threads of a row: four columns each
+        for (int i = tid; i < 32 * CT; i += 64 * NW) {
+            const int rr = i / CT, c = 4 * (i % CT);
+            if (row0 + rr >= nrow) continue;
+            float M = -INFINITY, w[NW], ls = 0.f;
+#pragma unroll
+            for (int j = 0; j < NW; ++j) M = fmaxf(M, stat[j * 32 + rr]);
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NW; ++j) {
+                const float mj = stat[j * 32 + rr], lj = stat[(NW + j) * 32 + rr];
+                w[j] = mj == -INFINITY ? (lj != lj ? lj : 0.f) : __builtin_amdgcn_exp2f(mj - M);
+                if (w[j] == 0.f) continue;   // a wave that saw no key
+                const f32x4 x = *reinterpret_cast<const f32x4*>(share + (j * 32 + rr) * LD + c);
+                ls += w[j] * lj;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] += w[j] * x[e];
+            }
+            const long long at = (long long)(rows.begin + (row0 + rr) / G) * a.H + hk * G + (row0 + rr) % G;
+            if (a.splits > 1) {
+                float* po = a.part_o + ((long long)blockIdx.y * a.s.Tq * a.H + at) * a.D;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < a.D) po[c + e] = o[e];
+                if (c == 0) {
+                    float* ml = a.part_ml + 2 * ((long long)blockIdx.y * a.s.Tq * a.H + at);
+                    ml[0] = M;
+                    ml[1] = ls;
+                }
+                continue;
+            }
+            const bool some = ls > 0.f || ls != ls;
+            const float inv = some ? 1.0f / ls : 0.f;
+            T* orow = (T*)a.o + at * a.D;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < a.D) orow[c + e] = (T)(o[e] * inv);
+            if (a.lse && c == 0) a.lse[at] = some ? (M + __builtin_amdgcn_logf(ls)) * LN2 : -INFINITY;
+        }
+        return;
+    }
     if (row >= nrow) return;
     const long long out_row = (long long)(rows.begin + tok) * a.H + head;
     if (a.splits > 1) {
@@ -190,38 +250,62 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_k
     if (a.lse && h == 0) a.lse[out_row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
-// joins the splits of a row: weights 2^(m_s - max m); one wave per row
+// joins the splits of a row: weights 2^(m_s - max m); one wave per row, lane s holds the weight of split s (at most 64)
 template <typename T>
 __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnArgs a) {
     const long long rows = a.s.Tq * a.H, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
-    for (int s = 0; s < a.splits; ++s) {
-        const float ms = a.part_ml[2 * (s * rows + row)], ls = a.part_ml[2 * (s * rows + row) + 1];
-        const float f = ms == -INFINITY ? (ls != ls ? ls : 0.f) : __builtin_amdgcn_exp2f(ms - m);
-        if (f == 0.f) continue;   // a split that sees no key
-        const float* po = a.part_o + (s * rows + row) * a.D;
-        l += f * ls;
-        if (lane < a.D) o0 += f * po[lane];
-        if (lane + 64 < a.D) o1 += f * po[lane + 64];
+    float ms = -INFINITY, ls = 0.f;
+    if (lane < a.splits) {
+        const float* ml = a.part_ml + 2 * (lane * rows + row);
+        ms = ml[0];
+        ls = ml[1];
     }
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    const float m = wave_max_f32(ms);
+    const float w = ms == -INFINITY ? (ls != ls ? ls : 0.f) : __builtin_amdgcn_exp2f(ms - m);   // 0: a split that sees no key
+    float l = 0.f, o0 = 0.f, o1 = 0.f;
+    const float* po = a.part_o + row * a.D;
+    for (int s = 0; s < a.splits; s += 4) {   // four splits' loads in flight
+        float x0[4], x1[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool on = s + j < a.splits;
+            x0[j] = on && lane < a.D ? po[(s + j) * rows * a.D + lane] : 0.f;
+            x1[j] = on && lane + 64 < a.D ? po[(s + j) * rows * a.D + lane + 64] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float f = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(w), min(s + j, 63)));
+            const float lj = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(ls), min(s + j, 63)));
+            if (s + j >= a.splits || f == 0.f) continue;
+            l += f * lj;
+            o0 += f * x0[j];
+            o1 += f * x1[j];
+        }
+    }
+    const bool some = l > 0.f || l != l;
+    const float inv = some ? 1.0f / l : 0.f;
     T* orow = (T*)a.o + row * a.D;
     if (lane < a.D) orow[lane] = (T)(o0 * inv);
     if (lane + 64 < a.D) orow[lane + 64] = (T)(o1 * inv);
-    if (a.lse && lane == 0) a.lse[row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    if (a.lse && lane == 0) a.lse[row] = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 constexpr int FWD_NW = 4;
 
-// How many parts a sequence's keys are split into: enough workgroups to fill the chip when there are few rows.  A part is no shorter than 256 keys on
-// average, so that what it writes (a row of fp32 per query row) stays small beside what it reads.
+// few rows: at most 32 (token, head of the group) rows per sequence on average
+bool few_rows(long long Tq, int n, int H, int Hk) { return Tq * (H / Hk) <= 32LL * n; }
+
+// How many parts a sequence's keys are split into: enough workgroups to fill the chip when there are few rows, and several times that many for few
+// rows, whose sequences may be of any length beside each other (16 single tokens against 161 to 32768 keys, 8 key heads of 128, bf16, up
+// to 512 / 1024 / 2048 / 4096 workgroups: 274 / 275 / 253 / 259 us; against 32768 each: 369 / 371 / 379 / 389 us, 5.8 to 5.5 TB/s).  A part is no shorter than 256 keys on average, so that what it writes (a
+// row of fp32 per query row) stays small beside what it reads.
 int split_count(long long Tq, long long Tk, int n, int H, int Hk) {
-    const long long wgs = ((Tq * (H / Hk) + 32 * FWD_NW - 1) / (32 * FWD_NW) > n ? (Tq * (H / Hk) + 32 * FWD_NW - 1) / (32 * FWD_NW) : n) * Hk;
-    if (wgs >= 512) return 1;
-    long long s = 1024 / (wgs > 0 ? wgs : 1);
+    const bool few = few_rows(Tq, n, H, Hk);
+    const long long bm = few ? 32 : 32 * FWD_NW, tiles = (Tq * (H / Hk) + bm - 1) / bm, wgs = (tiles > n ? tiles : n) * Hk;
+    if (wgs >= 512 && !few) return 1;
+    long long s = (few ? 2048 : 1024) / (wgs > 0 ? wgs : 1);
     const long long most = Tk / (n > 0 ? n : 1) / 256;
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -244,24 +328,34 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
     if (Tq == 0) return 0;
     const int splits = split_count(Tq, Tk, nseq, H, Hk), G = H / Hk;
     if (splits > 1 && !ws) return CASMTR_ERR_UNSUPPORTED;
-    const long long rows = Tq * H, wgs = slot_count(Tq, G, nseq, 32 * FWD_NW) * Hk;
+    const bool few = few_rows(Tq, nseq, H, Hk);
+    const long long rows = Tq * H, wgs = slot_count(Tq, G, nseq, few ? 32 : 32 * FWD_NW) * Hk;
     if (wgs > 0x7fffffffLL) return CASMTR_ERR_UNSUPPORTED;
     AttnArgs a{q, k, v, o, lse, ws, ws ? ws + (long long)splits * rows * D : nullptr, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk},
                qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits, scale * 1.44269504088896341f};
     ProfScope ps(CASMTR_PROF_GLUE, (hipStream_t)stream, "packed_attn_kernel");
     const bool ok = with_type(dtype, [&](auto tv) {
         typedef decltype(tv) T;
-        const dim3 grid((unsigned)wgs, (unsigned)splits), block(64 * FWD_NW);
-        constexpr int BN = sizeof(T) == 2 ? 64 : 32;   // the widest heads' tiles: 64 KB of LDS either way
-        const bool dma = TileDma<T, 128, 64, FWD_NW>::fits(k, kts, khs, D) && TileDma<T, 128, 64, FWD_NW>::fits(v, vts, vhs, D);
-#define FWD_LAUNCH(DP, BN)                                                                                                    \
-    do {                                                                                                                      \
-        if (dma) hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, FWD_NW, true>), grid, block, 0, (hipStream_t)stream, a);   \
-        else hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, FWD_NW, false>), grid, block, 0, (hipStream_t)stream, a);      \
+        const dim3 grid((unsigned)wgs, (unsigned)splits);
+        // LDS: at most 64 KB, two workgroups per CU (few rows of 128 columns in 16 bits with 128 KB, one workgroup: 379 -> 436 us as above);
+        // fp32 heads of more than 64 (32 for few rows) columns take 64 to 128 KB
+        constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+        typedef TileDma<T, 128, 128, FWD_NW> Dma;
+        const bool dma = Dma::fits(k, kts, khs, D) && Dma::fits(v, vts, vhs, D);
+#define FWD_LAUNCH(DP, BN, NW, FEW)                                                                                                  \
+    do {                                                                                                                             \
+        if (dma) hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, NW, true, FEW>), grid, dim3(64 * NW), 0, (hipStream_t)stream, a); \
+        else hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, NW, false, FEW>), grid, dim3(64 * NW), 0, (hipStream_t)stream, a);    \
     } while (0)
-        if (D <= 32) FWD_LAUNCH(32, 64);
-        else if (D <= 64) FWD_LAUNCH(64, 64);
-        else FWD_LAUNCH(128, BN);
+        if (few) {
+            if (D <= 32) FWD_LAUNCH(32, 128, 4, true);
+            else if (D <= 64) FWD_LAUNCH(64, 128, 4, true);
+            else FWD_LAUNCH(128, 64, 2, true);
+        } else {
+            if (D <= 32) FWD_LAUNCH(32, 64, FWD_NW, false);
+            else if (D <= 64) FWD_LAUNCH(64, 64, FWD_NW, false);
+            else FWD_LAUNCH(128, BN, FWD_NW, false);
+        }
 #undef FWD_LAUNCH
         if (splits > 1) hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
     });

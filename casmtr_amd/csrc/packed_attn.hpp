@@ -300,34 +300,45 @@ struct PackedSeqs {
     long long Tq, Tk;
 };
 struct Span { int begin, count; };
-// the rows of "sequence" s = -1 .. n: -1 and n are the rows before the first and behind the last one, which belong to none.  Whatever the
-// arrays hold, spans stay inside the tensors.
+// The rows of "sequence" s = -1 .. n: -1 and n are the rows before the first and behind the last one, which belong to none.  Whatever the
+// arrays hold, spans stay inside the tensors.  The loads are unconditional (indices clamped), so that those of a span and of both spans
+// of a sequence travel together: a workgroup's first tile waits for three round trips to memory, its place, its spans, its data.
 __device__ __forceinline__ int bound_of(const int* cu, int s, int n, long long T) {
-    if (s < 0) return 0;
-    return s > n ? (int)T : (int)max(0LL, min((long long)cu[s], T));
+    const int v = (int)max(0LL, min((long long)cu[max(0, min(s, n))], T));
+    return s < 0 ? 0 : s > n ? (int)T : v;
 }
 __device__ __forceinline__ Span span_of(const int* cu, int s, int n, long long T) {
-    const int b = bound_of(cu, s, n, T);
-    return {b, max(0, bound_of(cu, s + 1, n, T) - b)};
+    const int b = bound_of(cu, s, n, T), e = bound_of(cu, s + 1, n, T);
+    return {b, max(0, e - b)};
 }
 __device__ __forceinline__ Span keys_of(const PackedSeqs& p, int s) {
-    if (s < 0 || s >= p.n) return {0, 0};
+    const bool none = s < 0 || s >= p.n;
     Span k = span_of(p.cu_k, s, p.n, p.Tk);
-    if (p.len_k) k.count = max(0, min(k.count, p.len_k[s]));
-    return k;
+    if (p.len_k) {
+        const int used = p.n > 0 ? p.len_k[max(0, min(s, p.n - 1))] : 0;
+        k.count = max(0, min(k.count, used));
+    }
+    return none ? Span{0, 0} : k;
 }
 // Tiles of SIZE rows (a token counts `per` rows): sequence s owns the slots from bound(s) * per / SIZE + s + 1 on, which leaves it at least
 // as many as it has tiles, whatever the lengths.  So the host sizes the grid from the tensors' shapes alone -- it never waits for the
-// lengths -- and a workgroup finds its tile with a binary search; slots too many leave at once.
+// lengths -- and a workgroup looks its tile up; slots too many leave at once.
 __host__ __device__ __forceinline__ long long slot_count(long long T, int per, int n, int size) { return T * per / size + n + 2; }
 __device__ __forceinline__ int seq_of_slot(const int* cu, int n, long long T, int per, int size, long long slot, int* tile) {
-    int lo = -1, hi = n;   // the last s whose first slot is <= slot
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((long long)bound_of(cu, mid, n, T) * per / size + mid + 1 <= slot) lo = mid;
-        else hi = mid - 1;
+    // the last s whose first slot is <= slot; 64 candidates at a time, one per lane: one round trip up to 62 sequences, two up to 4000
+    const int lane = threadIdx.x & 63;
+    const auto first = [&](int s) { return (long long)bound_of(cu, s, n, T) * per / size + s + 1; };
+    int lo = -1, hi = n;
+    for (;;) {
+        const int step = (hi - lo) / 64 + 1;
+        const long long s = (long long)lo + (long long)lane * step;
+        const unsigned long long below = __ballot(s <= hi && (lane == 0 || first((int)min(s, (long long)hi)) <= slot));   // (lane 0: known)
+        lo += (63 - __builtin_clzll(below)) * step;
+        hi = (int)min((long long)hi, (long long)lo + step - 1);
+        if (step == 1) break;
     }
-    *tile = (int)(slot - ((long long)bound_of(cu, lo, n, T) * per / size + lo + 1));
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    *tile = (int)max(0LL, slot - first(lo));   // (never negative for non-decreasing bounds)
     return lo;
 }
 }  // namespace casmtr
