@@ -7,6 +7,7 @@ to the CPU.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 
@@ -32,7 +33,16 @@ def _ptr(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    """the current device's current HIP stream (torch.cuda.current_stream() builds a Stream object: 8 us against 0.2)"""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(device):
+    """the device guard, without its cost where `device` is the current one"""
+    return _SAME_DEVICE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _u8(mask):
@@ -755,7 +765,7 @@ _TOKEN_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _QUANT_TYPES = {torch.float8_e4m3fn: 1, torch.float8_e5m2: 2, torch.int8: 3}
 
 
-def _chk_tok(t, name, like=None, rows=False):
+def _chk_tok(t, name, like=None):
     """a token tensor: on the device, fp32 / fp16 / bf16, last axis contiguous; `like`: same device and type as that one"""
     if t is None:
         return None
@@ -765,13 +775,15 @@ def _chk_tok(t, name, like=None, rows=False):
         raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise RuntimeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
         raise RuntimeError(f"{name} must be contiguous along its last axis")
     return t
 
 
 def _rows(t, name):
     """[..., C] as (rows, C, row stride): the leading axes must collapse to one stride"""
+    if t.dim() == 2 and t.shape[1]:
+        return t.shape[0], t.shape[1], t.stride(0)
     if t.dim() < 1 or t.shape[-1] == 0:
         raise RuntimeError(f"{name} must be [..., C] with C >= 1")
     try:
@@ -801,7 +813,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_rstd=False):
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     h = torch.empty_like(y) if residual is not None else None
     rstd = torch.empty(R, device=x.device, dtype=torch.float32) if want_rstd else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         _lib.check(_lib.lib().casmtr_rms_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(y), _ptr(h), _ptr(rstd), None, R, C, xs, rs, float(eps),
                                                   _TOKEN_TYPES[x.dtype], _TOKEN_TYPES[weight.dtype], 0, 0, _stream()), "rms_norm_fwd")
     return (y, h, rstd) if want_rstd else (y, h)
@@ -820,7 +832,7 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn
     q = torch.empty(x.shape, device=x.device, dtype=dtype)
     scale = torch.empty(x.shape[:-1] if group is None else (*x.shape[:-1], C // 128), device=x.device, dtype=torch.float32)
     h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         _lib.check(_lib.lib().casmtr_rms_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(q), _ptr(h), None, _ptr(scale), R, C, xs, rs, float(eps),
                                                   _TOKEN_TYPES[x.dtype], _TOKEN_TYPES[weight.dtype], _QUANT_TYPES[dtype], group or 0, _stream()),
                    "rms_norm_fwd")
@@ -840,7 +852,7 @@ def rms_norm_bwd(dy, h, weight, rstd, dh=None):
     dw = torch.empty_like(weight)
     l = _lib.lib()
     ws = torch.empty(l.casmtr_rms_norm_bwd_ws_floats(R, C), device=h.device, dtype=torch.float32)
-    with torch.cuda.device(h.device):
+    with _on(h.device):
         _lib.check(l.casmtr_rms_norm_bwd(_ptr(dy), _ptr(dh), _ptr(h), _ptr(weight), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws), R, C, _rows(dy, "dy")[2],
                                          0 if dh is None else _rows(dh, "dh")[2], hs, _TOKEN_TYPES[h.dtype], _TOKEN_TYPES[weight.dtype], _stream()),
                    "rms_norm_bwd")
@@ -871,11 +883,13 @@ def rotary_freqs(dim, base=10000.0, factor=1.0, trained=None, axes=1, device="cu
 
 
 def _chk_heads(t, name, like=None):
-    """[T, H, D] token tensor whose heads are contiguous rows -> (token stride, head stride)"""
+    """[T, H, D] token tensor whose heads are contiguous rows -> its strides"""
+    st = t.stride()
+    if (t.is_cuda and len(st) == 3 and (st[2] == 1 or t.shape[2] <= 1) and t.dtype in _TOKEN_TYPES
+            and (like is None or (t.dtype == like.dtype and t.device == like.device))):
+        return st
     _chk_tok(t, name, like)
-    if t.dim() != 3:
-        raise RuntimeError(f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
-    return t.stride(0), t.stride(1)
+    raise RuntimeError(f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
 
 
 def rotary(q, k, positions, inv_freq, layout="half", gain=1.0, inverse=False):
@@ -889,7 +903,7 @@ def rotary(q, k, positions, inv_freq, layout="half", gain=1.0, inverse=False):
         raise RuntimeError(f"rotary: layout must be 'half' or 'interleaved', got {layout!r}")
     qs = _chk_heads(q, "q")
     T, Hq, D = q.shape
-    ks, Hk = (0, 0), 0
+    ks, Hk = (0, 0, 1), 0
     if k is not None:
         ks, Hk = _chk_heads(k, "k", q), k.shape[1]
         if k.shape[0] != T or k.shape[2] != D:
@@ -906,18 +920,18 @@ def rotary(q, k, positions, inv_freq, layout="half", gain=1.0, inverse=False):
         raise RuntimeError(f"rotary: 1 to min(D / 2, 1024) pairs (an even number with two positions per token), got {n} for D {D}")
     oq = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
     ok = torch.empty((T, Hk, D), device=q.device, dtype=q.dtype) if k is not None else None
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         _lib.check(_lib.lib().casmtr_rotary_fwd(_ptr(q), _ptr(k), _ptr(positions), _ptr(inv_freq), _ptr(oq), _ptr(ok), T, Hq, Hk, D, n, axes,
                                                 int(positions.dtype == torch.int64), int(layout == "interleaved"), float(gain), int(bool(inverse)),
-                                                *qs, *ks, _TOKEN_TYPES[q.dtype], _stream()), "rotary_fwd")
+                                                qs[0], qs[1], ks[0], ks[1], _TOKEN_TYPES[q.dtype], _stream()), "rotary_fwd")
     return oq, ok
 
 
 def _packed_args(q, k, v, cu_q, cu_k, len_k, scale):
     """checks of the packed attention's operands -> (cu_k, scale, sizes, strides)"""
     qs, ks, vs = _chk_heads(q, "q"), _chk_heads(k, "k", q), _chk_heads(v, "v", q)
-    (Tq, H, D), (Tk, Hk, _) = q.shape, k.shape
-    if k.shape != v.shape or k.shape[2] != D:
+    (Tq, H, D), (Tk, Hk, Dk), dev = q.shape, k.shape, q.device
+    if k.shape != v.shape or Dk != D:
         raise RuntimeError(f"packed_attn: k and v must be [keys, kv_heads, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
     if Hk < 1 or H < 1 or H % Hk:
         raise RuntimeError(f"packed_attn: {H} query heads do not share {Hk} key heads evenly")
@@ -928,15 +942,15 @@ def _packed_args(q, k, v, cu_q, cu_k, len_k, scale):
             raise RuntimeError("packed_attn: without cu_k the keys are the rows' own and k must have q's rows")
         cu_k = cu_q
     for t, n in ((cu_q, "cu_q"), (cu_k, "cu_k"), (len_k, "len_k")):
-        if t is not None and (_chk(t, n, torch.int32).dim() != 1 or t.device != q.device):
-            raise RuntimeError(f"{n} must be an int32 vector on {q.device}")
+        if t is not None and (_chk(t, n, torch.int32).dim() != 1 or t.device != dev):
+            raise RuntimeError(f"{n} must be an int32 vector on {dev}")
     n = cu_q.numel() - 1
     if n < 0 or cu_k.numel() != n + 1 or (len_k is not None and len_k.numel() != n):
         raise RuntimeError("packed_attn: cu_q and cu_k must have one more element than there are sequences, len_k as many")
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise RuntimeError(f"packed_attn: scale must be positive and finite, got {scale}")
-    return cu_k, scale, (Tq, Tk, n, H, Hk, D), (*qs, *ks, *vs)
+    return cu_k, scale, (Tq, Tk, n, H, Hk, D), (*qs[:2], *ks[:2], *vs[:2])
 
 
 def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, want_lse=False):
@@ -950,15 +964,16 @@ def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, 
     Scores, softmax statistics and sums are fp32; probabilities are rounded to the values' type for the product with them.  No host
     synchronisation; safe to capture into a HIP graph."""
     cu_k, scale, sizes, strides = _packed_args(q, k, v, cu_q, cu_k, len_k, scale)
-    Tq, Tk, n, H, Hk, D = sizes
-    out = torch.empty((Tq, H, D), device=q.device, dtype=q.dtype)
-    lse = torch.empty((Tq, H), device=q.device, dtype=torch.float32) if want_lse else None
+    dev, dt = q.device, q.dtype
+    out = torch.empty(q.shape, device=dev, dtype=dt)
+    lse = torch.empty(q.shape[:2], device=dev, dtype=torch.float32) if want_lse else None
     l = _lib.lib()
     wsf = l.casmtr_packed_attn_ws_floats(*sizes)
-    ws = torch.empty(wsf, device=q.device, dtype=torch.float32) if wsf else None
-    with torch.cuda.device(q.device):
-        _lib.check(l.casmtr_packed_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(ws), _ptr(cu_q), _ptr(cu_k), _ptr(len_k), *sizes, *strides,
-                                            scale, int(bool(causal)), _TOKEN_TYPES[q.dtype], _stream()), "packed_attn_fwd")
+    ws = torch.empty(wsf, device=dev, dtype=torch.float32) if wsf else None
+    with _on(dev):
+        rc = l.casmtr_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(ws), cu_q.data_ptr(), cu_k.data_ptr(),
+                                      _ptr(len_k), *sizes, *strides, scale, 1 if causal else 0, _TOKEN_TYPES[dt], _stream())
+    _lib.check(rc, "packed_attn_fwd")
     return (out, lse) if want_lse else out
 
 
@@ -975,7 +990,7 @@ def packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k=None, len_k=None, causal
     l = _lib.lib()
     wsf = l.casmtr_packed_attn_bwd_ws_floats(*sizes)
     ws = torch.empty(wsf, device=q.device, dtype=torch.float32) if wsf else None
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         _lib.check(l.casmtr_packed_attn_bwd(_ptr(grad), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), _ptr(cu_q),
                                             _ptr(cu_k), _ptr(len_k), *sizes, *strides, scale, int(bool(causal)), _TOKEN_TYPES[q.dtype], _stream()),
                    "packed_attn_bwd")
