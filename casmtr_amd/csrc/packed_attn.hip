@@ -96,8 +96,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packe
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (32 * b + 8 * (i >> 2) + (i & 3) >= lim) s[b][i] = -INFINITY;
+                        for (int i = 0; i < 16; ++i) s[b][i] = seen_or(s[b][i], -INFINITY, 32 * b + 8 * (i >> 2) + (i & 3), lim);
                 }
                 float mx = s[0][0];
 #pragma unroll

@@ -248,6 +248,13 @@ __device__ __forceinline__ float add_halves(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// `v` where x < limit, `hidden` elsewhere.  In bits, not as `if` or `?:`: those become control flow that the compiler merges with the wave-uniform
+// `if` around the masks, and then every tile pays for them.
+__device__ __forceinline__ float seen_or(float v, float hidden, int x, int limit) {
+    const unsigned m = (unsigned)((x - limit) >> 31);
+    return __uint_as_float((__float_as_uint(v) & m) | (__float_as_uint(hidden) & ~m));
+}
+
 // whether any of the wave's eight elements is infinite or NaN
 template <typename T>
 __device__ __forceinline__ bool any_not_finite(const frag_t<T>& f) {

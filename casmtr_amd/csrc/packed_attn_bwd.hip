@@ -123,8 +123,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
                 if (hidden) {
                     const int lim = limit - t * BN - 4 * h;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (32 * b + 8 * (i >> 2) + (i & 3) >= lim) s[i] = 0.f;
+                    for (int i = 0; i < 16; ++i) s[i] = seen_or(s[i], 0.f, 32 * b + 8 * (i >> 2) + (i & 3), lim);
                 }
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
@@ -199,11 +198,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
         const int hd = hk * G + n / per, t = t0 + n % per;
         if (tid < BM) {
             const int tok = t * BM + tid;
-            sl = sd = 0.f;
+            sl = INFINITY;   // a row that is not there or sees nothing: its probabilities are exactly 0
+            sd = 0.f;
             if (tok < rows.count) {
                 const long long at = (long long)(rows.begin + tok) * a.H + hd;
                 const float x = a.lse[at];
-                sl = x == -INFINITY ? 0.f : x * LOG2E;
+                sl = x == -INFINITY ? INFINITY : x * LOG2E;
                 sd = a.delta[at];
             }
         }
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
             __syncthreads();
             if (n + 1 < turns) fetch(n + 1, stage ^ 1);
             if ((t + 1) * BM <= wave_first) return;
-            const bool hidden = t * BM < wave_all || (t + 1) * BM > rows.count;
+            const bool hidden = t * BM < wave_all;
             const char *qs = qg.first(stage), *gs = qg.second(stage);
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
@@ -247,11 +247,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
                 // element n & 7 of half n >> 3 of step tt stands for token t BM + 32 b + 16 tt + 8 (n >> 2 & 1) + 4 (n >> 3) + (n & 3)
                 const int tok0 = t * BM + 32 * b;
                 if (hidden) {
-                    const int lo = first - tok0 - 4 * h, hi = rows.count - tok0 - 4 * h;
+                    const int lo = first - tok0 - 4 * h;   // (rows behind the last are excluded by their lse)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int x = 8 * (i >> 2) + (i & 3);
-                        if (x < lo || x >= hi) { s[i] = 0.f; dp[i] = 0.f; }
+                        s[i] = seen_or(s[i], 0.f, -1 - x, -lo);
+                        dp[i] = seen_or(dp[i], 0.f, -1 - x, -lo);
                     }
                 }
 #pragma unroll
