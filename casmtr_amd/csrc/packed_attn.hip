@@ -3,6 +3,9 @@
 // Row i of a sequence with nq rows and nk keys sees all keys, or, causal, the keys j <= i + nk - nq.  A row that sees none gives 0 and -inf.
 // Query heads share key heads in groups of G = H / Hk.
 //
+// fp32 runs as three bf16 terms (x3_t) -- 8 x 43264 rows x 676 keys, 4 heads of 32: 825 us (145 TFLOP/s) against 1118 us on the fp32 matrix
+// instructions, whose 154 TFLOP/s bound it --, except for few rows, where the reads bound it.
+//
 // One pass over the keys with the running maximum and sum of the softmax.  A tile's rows are (token, head of the group) pairs, token-major, so
 // all G heads of a key head use one copy of its keys, and a single token of G heads is one tile.  A workgroup has four waves of 32 rows; K and V
 // tiles of BN keys go through LDS in two stages: the next tile's loads are in flight while this one is multiplied, one barrier per tile.
@@ -28,8 +31,8 @@ constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a m
 // FEW (few rows, long keys): a workgroup has 32 rows, its waves take 32 keys each of a tile and are joined in LDS at the end.  With 128 rows per
 // workgroup a tile takes each wave the whole way through 64 keys, for nothing where three of four waves have no rows of their own.
 template <typename T, int DP, int BN, int NW, bool DMA, bool FEW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
-    typedef Tile<T, DP> L;
+__global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1 && DP <= 64)) ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
+    typedef Tile<T, DP, BN> L;
     static_assert(!FEW || BN == 32 * NW, "one block of keys per wave");
     constexpr int BM = FEW ? 32 : 32 * NW, KS = DP / 16, NB = FEW ? 1 : BN / 32, DB = DP / 32;
     __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BN, NW, DMA>::BYTES];
@@ -56,13 +59,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packe
     }
     TilePair<T, DP, BN, NW, DMA> kv;
     kv.init(smem, tid, wave, a.kts, a.vts, a.D);
-    kv.of((const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
+    kv.of((const store_t<T>*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const store_t<T>*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
     if (t0 < t1) kv.fetch(t0, 0);
     frag_t<T> qf[KS];
     {
-        const T* qr = (const T*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
+        const store_t<T>* qr = (const store_t<T>*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = load_frag(qr, s, h, a.D);
+        for (int s = 0; s < KS; ++s) qf[s] = load_frag<T>(qr, s, h, a.D);
     }
     f32x16 acc[DB];
     float m, l;
@@ -89,7 +92,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packe
                 for (int b = 0; b < NB; ++b) {
                     s[b] = zero16();
 #pragma unroll
-                    for (int st = 0; st < KS; ++st) s[b] = mma(L::rows(ks, wkey + 32 * b + r, st, h), qf[st], s[b]);
+                    for (int st = 0; st < KS; ++st) {
+                        const frag_t<T> kf = L::rows(ks, wkey + 32 * b + r, st, h);
+                        s[b] = GUARD ? mma_any<T>(kf, qf[st], s[b]) : mma(kf, qf[st], s[b]);
+                    }
                 }
                 if (hidden) {
                     const int lim = limit - key0 - 4 * h;
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packe
     pass(std::false_type{});
     // Hidden keys are weighted with exact zeros, so an infinity or NaN among hidden values is the only way by which one can reach a row that
     // does not see it -- and then the row's sum is not finite.  Rare enough to do it again, carefully, when that is seen.
-    if (a.s.causal) {
+    if (a.s.causal || std::is_same<T, x3_t>::value) {   // (three terms turn an infinity into NaN: that is done again too)
         float worst = 0.f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -201,10 +207,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packe
             }
             const bool some = ls > 0.f || ls != ls;
             const float inv = some ? 1.0f / ls : 0.f;
-            T* orow = (T*)a.o + at * a.D;
+            store_t<T>* orow = (store_t<T>*)a.o + at * a.D;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < a.D) orow[c + e] = (T)(o[e] * inv);
+                if (c + e < a.D) orow[c + e] = (store_t<T>)(o[e] * inv);
             if (a.lse && c == 0) a.lse[at] = some ? (M + __builtin_amdgcn_logf(ls)) * LN2 : -INFINITY;
         }
         return;
@@ -230,16 +236,17 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && !FEW ? 2 : 1) void packe
         return;
     }
     const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-    T* orow = (T*)a.o + out_row * a.D;
+    store_t<T>* orow = (store_t<T>*)a.o + out_row * a.D;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * h;
-            typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            typedef store_t<T> S;
+            typedef S T4 __attribute__((ext_vector_type(4), aligned(sizeof(S))));
             T4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[d][4 * g + e] * inv);
+            for (int e = 0; e < 4; ++e) v[e] = (S)(acc[d][4 * g + e] * inv);
             if (c + 4 <= a.D) *reinterpret_cast<T4*>(orow + c) = v;
             else
 #pragma unroll
@@ -338,7 +345,6 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
         const dim3 grid((unsigned)wgs, (unsigned)splits);
         // LDS: at most 64 KB, two workgroups per CU (few rows of 128 columns in 16 bits with 128 KB, one workgroup: 379 -> 436 us as above);
         // fp32 heads of more than 64 (32 for few rows) columns take 64 to 128 KB
-        constexpr int BN = sizeof(T) == 2 ? 64 : 32;
         typedef TileDma<T, 128, 128, FWD_NW> Dma;
         const bool dma = Dma::fits(k, kts, khs, D) && Dma::fits(v, vts, vhs, D);
 #define FWD_LAUNCH(DP, BN, NW, FEW)                                                                                                  \
@@ -350,10 +356,15 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
             if (D <= 32) FWD_LAUNCH(32, 128, 4, true);
             else if (D <= 64) FWD_LAUNCH(64, 128, 4, true);
             else FWD_LAUNCH(128, 64, 2, true);
-        } else {
+        } else if constexpr (sizeof(T) == 2) {
             if (D <= 32) FWD_LAUNCH(32, 64, FWD_NW, false);
             else if (D <= 64) FWD_LAUNCH(64, 64, FWD_NW, false);
-            else FWD_LAUNCH(128, BN, FWD_NW, false);
+            else FWD_LAUNCH(128, 64, FWD_NW, false);
+        } else {
+            const dim3 block(64 * FWD_NW);
+            if (D <= 32) hipLaunchKernelGGL((packed_attn_kernel<x3_t, 32, 64, FWD_NW, false, false>), grid, block, 0, (hipStream_t)stream, a);
+            else if (D <= 64) hipLaunchKernelGGL((packed_attn_kernel<x3_t, 64, 32, FWD_NW, false, false>), grid, block, 0, (hipStream_t)stream, a);
+            else hipLaunchKernelGGL((packed_attn_kernel<x3_t, 128, 32, FWD_NW, false, false>), grid, block, 0, (hipStream_t)stream, a);
         }
 #undef FWD_LAUNCH
         if (splits > 1) hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);

@@ -18,8 +18,16 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;   // 16 bytes at any element
 
+// x3_t: fp32 data multiplied as three bf16 terms, x = x0 + x1 + x2 (8 bits each: the 24 bits of x), of whose nine products the six largest are
+// kept: what is dropped is below 2^-24 of the product, as the rounding of an fp32 product is.  Six bf16 matrix instructions of 32 cycles
+// stand for eight fp32 ones of 64.  (Values beyond 2^128 (1 - 2^-9) count as infinite.)
+struct x3_t {};
 template <typename T> struct FragOf { typedef T type __attribute__((ext_vector_type(8))); };
+template <> struct FragOf<x3_t> { struct type { FragOf<bf16_t>::type t[3]; }; };
 template <typename T> using frag_t = typename FragOf<T>::type;
+template <typename T> struct StoreOf { typedef T type; };   // the type in memory
+template <> struct StoreOf<x3_t> { typedef float type; };
+template <typename T> using store_t = typename StoreOf<T>::type;
 
 __device__ __forceinline__ f32x16 mma(const frag_t<bf16_t>& a, const frag_t<bf16_t>& b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -32,6 +40,25 @@ __device__ __forceinline__ f32x16 mma(const frag_t<float>& a, const frag_t<float
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
     return c;
 }
+__device__ __forceinline__ f32x16 mma(const frag_t<x3_t>& a, const frag_t<x3_t>& b, f32x16 c) {   // the small products first
+    c = mma(a.t[2], b.t[0], c);
+    c = mma(a.t[0], b.t[2], c);
+    c = mma(a.t[1], b.t[1], c);
+    c = mma(a.t[1], b.t[0], c);
+    c = mma(a.t[0], b.t[1], c);
+    return mma(a.t[0], b.t[0], c);
+}
+__device__ __forceinline__ frag_t<x3_t> split3(const float (&x)[8]) {
+    frag_t<x3_t> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f.t[0][e] = (bf16_t)x[e];
+        const float r = x[e] - (float)f.t[0][e];
+        f.t[1][e] = (bf16_t)r;
+        f.t[2][e] = (bf16_t)(r - (float)f.t[1][e]);
+    }
+    return f;
+}
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -42,7 +69,7 @@ __device__ __forceinline__ f32x16 zero16() {
 // An LDS tile of ROWS x DP elements in 16-byte chunks.  Rows are read at one chunk by 32 lanes (ds_read_b128) and, transposed, four rows x four
 // chunks by 32 lanes (16-bit) or two rows x eight chunks by 64 lanes (fp32); the exclusive-or below puts the chunks of each such access on
 // different banks (256 bytes = all 64 banks = one "line" of 16 chunks; rows shorter than that share a line).
-template <typename T, int DP>
+template <typename T, int DP, int ROWS>
 struct Tile {
     static constexpr int EPC = 16 / (int)sizeof(T);          // elements of a chunk
     static constexpr int CPR = DP / EPC;                     // chunks of a row
@@ -113,6 +140,19 @@ struct Tile {
     }
 };
 
+// x3_t: one tile per term, one behind the other
+template <int DP, int ROWS>
+struct Tile<x3_t, DP, ROWS> {
+    typedef Tile<bf16_t, DP, ROWS> P;
+    static constexpr int RB = 3 * P::RB, PLANE = ROWS * P::RB;
+    static __device__ __forceinline__ frag_t<x3_t> rows(const char* tile, int row, int s, int h) {
+        return {{P::rows(tile, row, s, h), P::rows(tile + PLANE, row, s, h), P::rows(tile + 2 * PLANE, row, s, h)}};
+    }
+    static __device__ __forceinline__ frag_t<x3_t> cols(const char* tile, int row0, int col0, int lane) {
+        return {{P::cols(tile, row0, col0, lane), P::cols(tile + PLANE, row0, col0, lane), P::cols(tile + 2 * PLANE, row0, col0, lane)}};
+    }
+};
+
 // 16 bytes of a row from column col on; columns from D on are zero
 template <typename T>
 __device__ __forceinline__ u32x4 load_chunk(const T* row, int col, int D) {
@@ -127,14 +167,22 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int col, int D) {
 }
 // the fragment of a row held in global memory: columns 16 s + 8 h ..
 template <typename T>
-__device__ __forceinline__ frag_t<T> load_frag(const T* row, int s, int h, int D) {
+__device__ __forceinline__ frag_t<T> load_frag(const store_t<T>* row, int s, int h, int D) {
     frag_t<T> f;
     const int col = 16 * s + 8 * h;
-    const u32x4 a = load_chunk(row, col, D);
-    __builtin_memcpy(&f, &a, 16);
-    if constexpr (sizeof(T) == 4) {
-        const u32x4 b = load_chunk(row, col + 4, D);
-        __builtin_memcpy(reinterpret_cast<char*>(&f) + 16, &b, 16);
+    if constexpr (std::is_same<T, x3_t>::value) {
+        float x[8];
+        const u32x4 a = load_chunk(row, col, D), b = load_chunk(row, col + 4, D);
+        __builtin_memcpy(x, &a, 16);
+        __builtin_memcpy(x + 4, &b, 16);
+        f = split3(x);
+    } else {
+        const u32x4 a = load_chunk(row, col, D);
+        __builtin_memcpy(&f, &a, 16);
+        if constexpr (sizeof(T) == 4) {
+            const u32x4 b = load_chunk(row, col + 4, D);
+            __builtin_memcpy(reinterpret_cast<char*>(&f) + 16, &b, 16);
+        }
     }
     return f;
 }
@@ -145,7 +193,7 @@ __device__ __forceinline__ frag_t<T> load_frag(const T* row, int s, int h, int D
 // overlap.  Inline asm, so that the compiler does not drain the loads in flight before every LDS read: the kernels wait with glds_wait().
 template <typename T, int DP, int ROWS, int NW>
 struct TileDma {
-    typedef Tile<T, DP> L;
+    typedef Tile<T, DP, ROWS> L;
     static constexpr int N = ROWS * L::CPR / (64 * NW);   // instructions per wave
     unsigned voff[N];
     unsigned row_bytes, width;
@@ -183,7 +231,7 @@ struct TileDma {
 // DMA: straight into LDS; otherwise (rows that are not 16-byte aligned) through registers, written when the tile is due.
 template <typename T, int DP, int ROWS, int NW, bool DMA>
 struct TilePair {
-    typedef Tile<T, DP> L;
+    typedef Tile<T, DP, ROWS> L;
     static constexpr int NT = 64 * NW, NCH = ROWS * L::CPR / NT, TB = ROWS * L::RB, BYTES = 4 * TB;
     static_assert(ROWS * L::CPR % NT == 0, "whole chunks per thread");
     char* smem;
@@ -230,13 +278,69 @@ struct TilePair {
     }
 };
 
+// x3_t: fp32 rows through registers, split on the way into LDS
+template <int DP, int ROWS, int NW>
+struct TilePair<x3_t, DP, ROWS, NW, false> {
+    typedef Tile<x3_t, DP, ROWS> L;
+    typedef Tile<bf16_t, DP, ROWS> P;
+    static constexpr int NT = 64 * NW, N = ROWS * P::CPR / NT, TB = 3 * L::PLANE, BYTES = 4 * TB;
+    static_assert(ROWS * P::CPR % NT == 0, "whole chunks per thread");
+    char* smem;
+    const float *a, *b;
+    long long as, bs;
+    int count, D, tid;
+    u32x4 ar[2 * N], br[2 * N];
+    __device__ __forceinline__ void init(char* smem_, int tid_, int, long long as_, long long bs_, int D_) { smem = smem_; tid = tid_; as = as_; bs = bs_; D = D_; }
+    __device__ __forceinline__ void of(const float* a_, const float* b_, int count_) { a = a_; b = b_; count = count_; }
+    __device__ __forceinline__ const char* first(int stage) const { return smem + 2 * stage * TB; }
+    __device__ __forceinline__ const char* second(int stage) const { return smem + (2 * stage + 1) * TB; }
+    __device__ __forceinline__ void fetch(int t, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = tid + NT * i, rr = t * ROWS + id / P::CPR, c = (id % P::CPR) * 8;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                ar[2 * i + j] = u32x4{0, 0, 0, 0};
+                br[2 * i + j] = u32x4{0, 0, 0, 0};
+                if (rr < count && c + 4 * j < D) {
+                    ar[2 * i + j] = load_chunk(a + (long long)rr * as, c + 4 * j, D);
+                    br[2 * i + j] = load_chunk(b + (long long)rr * bs, c + 4 * j, D);
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void put(char* tile, int o, const u32x4& lo, const u32x4& hi) {
+        float x[8];
+        __builtin_memcpy(x, &lo, 16);
+        __builtin_memcpy(x + 4, &hi, 16);
+        const frag_t<x3_t> f = split3(x);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<frag_t<bf16_t>*>(tile + j * L::PLANE + o) = f.t[j];
+    }
+    __device__ __forceinline__ void arrived(int stage) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = tid + NT * i, o = P::off(id / P::CPR, id % P::CPR);
+            put(smem + 2 * stage * TB, o, ar[2 * i], ar[2 * i + 1]);
+            put(smem + (2 * stage + 1) * TB, o, br[2 * i], br[2 * i + 1]);
+        }
+    }
+};
+
 // registers 8 t .. 8 t + 7 of a result as the next product's operand
 template <typename T>
 __device__ __forceinline__ frag_t<T> to_frag(const f32x16& c, int t) {
-    frag_t<T> f;
+    if constexpr (std::is_same<T, x3_t>::value) {
+        float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (T)c[8 * t + e];
-    return f;
+        for (int e = 0; e < 8; ++e) x[e] = c[8 * t + e];
+        return split3(x);
+    } else {
+        frag_t<T> f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (T)c[8 * t + e];
+        return f;
+    }
 }
 
 __device__ __forceinline__ float max_halves(float v) {   // max / sum with the other half of the wave
@@ -274,29 +378,61 @@ __device__ __forceinline__ bool any_not_finite(const frag_t<T>& f) {
 // half n >> 3 stands for.
 template <typename T, typename Sees>
 __device__ __forceinline__ f32x16 mma_hidden(const frag_t<T>& a, const frag_t<T>& b, f32x16 c, int h, Sees&& sees) {
-    if (__builtin_expect(!any_not_finite<T>(a), 1)) return mma(a, b, c);
+    constexpr bool X3 = std::is_same<T, x3_t>::value;
+    const auto& a0 = [&]() -> const auto& { if constexpr (X3) return a.t[0]; else return a; }();   // (of the terms, the first says it)
+    typedef std::conditional_t<X3, bf16_t, T> E;
+    if (__builtin_expect(!any_not_finite<E>(a0), 1)) return mma(a, b, c);
     frag_t<T> fin;
     unsigned odd = 0;   // this lane's elements that are not finite
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const bool ok = __builtin_fabsf((float)a[e]) < INFINITY;
-        fin[e] = ok ? a[e] : (T)0.f;
+        const bool ok = __builtin_fabsf((float)a0[e]) < INFINITY;
+        if constexpr (X3) {
+#pragma unroll
+            for (int j = 0; j < 3; ++j) fin.t[j][e] = ok ? a.t[j][e] : (E)0.f;
+        } else fin[e] = ok ? a[e] : (E)0.f;
         odd |= (ok ? 0u : 1u) << (8 * h + e);
     }
     c = mma(fin, b, c);
     for (int n = 0; n < 16; ++n) {
         if (!__any((odd >> n) & 1u)) continue;
-        frag_t<T> a1, b1;
+        frag_t<E> a1, b1;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool on = n == 8 * h + e;
-            a1[e] = on && ((odd >> n) & 1u) ? a[e] : (T)0.f;
-            b1[e] = on ? b[e] : (T)0.f;
+            a1[e] = on && ((odd >> n) & 1u) ? a0[e] : (E)0.f;
+            if constexpr (X3) b1[e] = on ? b.t[0][e] : (E)0.f;
+            else b1[e] = on ? b[e] : (E)0.f;
         }
         const f32x16 d = mma(a1, b1, c);
         if (sees(n)) c = d;
     }
     return c;
+}
+// c += A B as the formula has it where either holds infinities or NaN.  Of three terms the second and third of an infinity are NaN: such
+// elements are multiplied by their first term alone.
+template <typename T>
+__device__ __forceinline__ f32x16 mma_any(const frag_t<T>& a, const frag_t<T>& b, f32x16 c) {
+    if constexpr (!std::is_same<T, x3_t>::value) return mma(a, b, c);
+    else {
+        if (!any_not_finite<bf16_t>(a.t[0]) && !any_not_finite<bf16_t>(b.t[0])) return mma(a, b, c);
+        frag_t<x3_t> fa, fb;
+        frag_t<bf16_t> oa, ob;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool ka = __builtin_fabsf((float)a.t[0][e]) < INFINITY, kb = __builtin_fabsf((float)b.t[0][e]) < INFINITY;
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                fa.t[j][e] = ka ? a.t[j][e] : (bf16_t)0.f;
+                fb.t[j][e] = kb ? b.t[j][e] : (bf16_t)0.f;
+            }
+            oa[e] = ka ? (bf16_t)0.f : a.t[0][e];
+            ob[e] = kb ? (bf16_t)0.f : b.t[0][e];
+        }
+        c = mma(fa, fb, c);
+        c = mma(oa, b.t[0], c);
+        return mma(fa.t[0], ob, c);
+    }
 }
 
 // ---- sequences

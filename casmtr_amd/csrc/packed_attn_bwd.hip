@@ -54,8 +54,8 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&acc)[DB]) {
 
 // dq: a workgroup's rows are (token, head) pairs as in the forward kernel
 template <typename T, int DP, int BN, int NW, bool DMA>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_dq_kernel(const BwdArgs a) {
-    typedef Tile<T, DP> L;
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <= 64) ? 2 : 1) void packed_attn_dq_kernel(const BwdArgs a) {
+    typedef Tile<T, DP, BN> L;
     constexpr int BM = 32 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
     __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BN, NW, DMA>::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
@@ -76,15 +76,19 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
     frag_t<T> qf[KS], gf[KS];
     float delta = 0.f;
     {
-        const T* qr = (const T*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
-        const T *gr = (const T*)a.g + out_row * a.D, *orow = (const T*)a.o + out_row * a.D;
+        const store_t<T>* qr = (const store_t<T>*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
+        const store_t<T> *gr = (const store_t<T>*)a.g + out_row * a.D, *orow = (const store_t<T>*)a.o + out_row * a.D;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            qf[s] = load_frag(qr, s, h, a.D);
-            gf[s] = load_frag(gr, s, h, a.D);
-            const frag_t<T> of = load_frag(orow, s, h, a.D);
+            qf[s] = load_frag<T>(qr, s, h, a.D);
+            gf[s] = load_frag<T>(gr, s, h, a.D);
+            float x[8], y[8];
+            const int c = 16 * s + 8 * h, n = a.D - c;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)gf[s][e], (float)of[e], delta);
+            for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.f;
+            if (n > 0) { load_n(gr + c, x, n); load_n(orow + c, y, n); }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
         }
     }
     delta = add_halves(delta);
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
     f32x16 acc[DB];
     TilePair<T, DP, BN, NW, DMA> kv;
     kv.init(smem, tid, wave, a.kts, a.vts, a.D);
-    kv.of((const T*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const T*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
+    kv.of((const store_t<T>*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const store_t<T>*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
     const auto pass = [&](auto guard) {
         constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
@@ -112,8 +116,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
-                    s = mma(L::rows(ks, 32 * b + r, st, h), qf[st], s);
-                    dp = mma(L::rows(vs, 32 * b + r, st, h), gf[st], dp);
+                    const frag_t<T> kf = L::rows(ks, 32 * b + r, st, h), vf = L::rows(vs, 32 * b + r, st, h);
+                    s = GUARD ? mma_any<T>(kf, qf[st], s) : mma(kf, qf[st], s);
+                    dp = GUARD ? mma_any<T>(vf, gf[st], dp) : mma(vf, gf[st], dp);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -144,17 +149,17 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void packed_attn_d
         }
     };
     pass(std::false_type{});
-    if (a.s.causal) {   // as in the forward kernel: a sum that is not finite may have met a hidden infinity
+    if (a.s.causal || std::is_same<T, x3_t>::value) {   // as in the forward kernel: a sum that is not finite may have met a hidden infinity
         if (__syncthreads_or(not_finite(acc))) pass(std::true_type{});
     }
-    if (row < nrow) store_row<T, DB>((T*)a.dq + out_row * a.D, acc, h, a.D, a.scale);
+    if (row < nrow) store_row<store_t<T>, DB>((store_t<T>*)a.dq + out_row * a.D, acc, h, a.D, a.scale);
 }
 
 // dk, dv: a workgroup owns BN = 32 NW keys of one key head, a wave 32 of them (K and V stay in its registers), and walks the rows of the heads that
 // share it, head by head in tiles of BM tokens
 template <typename T, int DP, int BM, int NW, bool DMA>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void packed_attn_dkv_kernel(const BwdArgs a) {
-    typedef Tile<T, DP> L;
+__global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T) == 1 && DP <= 32) ? 2 : 1) void packed_attn_dkv_kernel(const BwdArgs a) {
+    typedef Tile<T, DP, BM> L;
     constexpr int BN = 32 * NW, KS = DP / 16, MB = BM / 32, DB = DP / 32;
     static_assert(BM <= 64 * NW, "a thread stages one row's statistics");
     __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BM, NW, DMA>::BYTES];
@@ -175,12 +180,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
     const int kc = max(0, min(key, keys.count - 1));
     frag_t<T> kf[KS], vf[KS];
     {
-        const T* kr = (const T*)a.k + (long long)(keys.begin + kc) * a.kts + hk * a.khs;
-        const T* vr = (const T*)a.v + (long long)(keys.begin + kc) * a.vts + hk * a.vhs;
+        const store_t<T>* kr = (const store_t<T>*)a.k + (long long)(keys.begin + kc) * a.kts + hk * a.khs;
+        const store_t<T>* vr = (const store_t<T>*)a.v + (long long)(keys.begin + kc) * a.vts + hk * a.vhs;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            kf[s] = load_frag(kr, s, h, keys.count > 0 ? a.D : 0);
-            vf[s] = load_frag(vr, s, h, keys.count > 0 ? a.D : 0);
+            kf[s] = load_frag<T>(kr, s, h, keys.count > 0 ? a.D : 0);
+            vf[s] = load_frag<T>(vr, s, h, keys.count > 0 ? a.D : 0);
         }
     }
     f32x16 dk[DB], dv[DB];
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
                 sd = a.delta[at];
             }
         }
-        qg.of((const T*)a.q + (long long)rows.begin * a.qts + hd * a.qhs, (const T*)a.g + ((long long)rows.begin * a.H + hd) * a.D, rows.count);
+        qg.of((const store_t<T>*)a.q + (long long)rows.begin * a.qts + hd * a.qhs, (const store_t<T>*)a.g + ((long long)rows.begin * a.H + hd) * a.D, rows.count);
         qg.fetch(t, stage);
     };
     const auto pass = [&](auto guard) {
@@ -230,8 +235,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
-                    s = mma(L::rows(qs, 32 * b + r, st, h), kf[st], s);
-                    dp = mma(L::rows(gs, 32 * b + r, st, h), vf[st], dp);
+                    const frag_t<T> qf = L::rows(qs, 32 * b + r, st, h), gf = L::rows(gs, 32 * b + r, st, h);
+                    s = GUARD ? mma_any<T>(qf, kf[st], s) : mma(qf, kf[st], s);
+                    dp = GUARD ? mma_any<T>(gf, vf[st], dp) : mma(gf, vf[st], dp);
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
@@ -284,7 +290,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
         }
     };
     pass(std::false_type{});
-    if (a.s.causal) {
+    if (a.s.causal || std::is_same<T, x3_t>::value) {
         if (__syncthreads_or(not_finite(dk) || not_finite(dv))) pass(std::true_type{});
     }
     if (key >= share.count) return;
@@ -300,8 +306,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void p
         store_row<float, DB>(part + n, dv, h, a.D, 1.f);
         return;
     }
-    store_row<T, DB>((T*)a.dk + out_row * a.D, dk, h, a.D, a.scale);
-    store_row<T, DB>((T*)a.dv + out_row * a.D, dv, h, a.D, 1.f);
+    store_row<store_t<T>, DB>((store_t<T>*)a.dk + out_row * a.D, dk, h, a.D, a.scale);
+    store_row<store_t<T>, DB>((store_t<T>*)a.dv + out_row * a.D, dv, h, a.D, 1.f);
 }
 
 // dk and dv as the sums of their splits, in order
@@ -357,25 +363,29 @@ extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* 
     ProfScope ps(CASMTR_PROF_GLUE, (hipStream_t)stream, "packed_attn_dq_kernel, packed_attn_dkv_kernel");
     with_type(dtype, [&](auto tv) {
         typedef decltype(tv) T;
-        const dim3 block(64 * BWD_NW), kgrid((unsigned)kwgs, (unsigned)splits);
+        const dim3 block(64 * BWD_NW), qgrid((unsigned)qwgs), kgrid((unsigned)kwgs, (unsigned)splits);
         const hipStream_t st = (hipStream_t)stream;
-        constexpr int W = sizeof(T) == 2 ? 64 : 32;   // the widest head's tiles: 64 KB of LDS either way
         typedef TileDma<T, 128, 64, BWD_NW> Dma;
         const bool kdma = Dma::fits(k, kts, khs, D) && Dma::fits(v, vts, vhs, D), qdma = Dma::fits(q, qts, qhs, D) && Dma::fits(g, (long long)H * D, D, D);
-#define BWD_LAUNCH(DP, TILE, RTILE)                                                                                                    \
-    do {                                                                                                                               \
-        if (Tq > 0) {                                                                                                                  \
-            if (kdma) hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, TILE, BWD_NW, true>), dim3((unsigned)qwgs), block, 0, st, a);   \
-            else hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, TILE, BWD_NW, false>), dim3((unsigned)qwgs), block, 0, st, a);       \
-        }                                                                                                                              \
-        if (Tk > 0) {                                                                                                                  \
-            if (qdma) hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, RTILE, BWD_NW, true>), kgrid, block, 0, st, a); \
-            else hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, RTILE, BWD_NW, false>), kgrid, block, 0, st, a);     \
-        }                                                                                                                              \
+        // E: the element as the kernel multiplies it (x3_t: fp32 in three terms, staged through registers at any alignment)
+#define BWD_LAUNCH(KERNEL, E, DP, TILE, DMA, GRID)                                                                      \
+    do {                                                                                                                \
+        constexpr bool CAN = sizeof(E) != 1;                                                                            \
+        if (CAN && DMA) hipLaunchKernelGGL((KERNEL<E, DP, TILE, BWD_NW, CAN>), GRID, block, 0, st, a);                  \
+        else hipLaunchKernelGGL((KERNEL<E, DP, TILE, BWD_NW, false>), GRID, block, 0, st, a);                           \
     } while (0)
-        if (D <= 32) BWD_LAUNCH(32, 64, 64);
-        else if (D <= 64) BWD_LAUNCH(64, 64, W);
-        else BWD_LAUNCH(128, W, 32);
+        constexpr bool WIDE = sizeof(T) == 4;
+        typedef std::conditional_t<WIDE, x3_t, T> E;
+        if (Tq > 0) {
+            if (D <= 32) BWD_LAUNCH(packed_attn_dq_kernel, E, 32, 64, kdma, qgrid);
+            else if (D <= 64) BWD_LAUNCH(packed_attn_dq_kernel, E, 64, (WIDE ? 32 : 64), kdma, qgrid);
+            else BWD_LAUNCH(packed_attn_dq_kernel, E, 128, (WIDE ? 32 : 64), kdma, qgrid);
+        }
+        if (Tk > 0) {
+            if (D <= 32) BWD_LAUNCH(packed_attn_dkv_kernel, E, 32, 64, qdma, kgrid);
+            else if (D <= 64) BWD_LAUNCH(packed_attn_dkv_kernel, E, 64, (WIDE ? 32 : 64), qdma, kgrid);
+            else BWD_LAUNCH(packed_attn_dkv_kernel, T, 128, 32, qdma, kgrid);   // fp32 terms of K and V do not fit the registers here: 95 against 124 TFLOP/s
+        }
 #undef BWD_LAUNCH
         if (splits > 1 && Tk > 0)
             hipLaunchKernelGGL((packed_attn_dkv_join_kernel<T>), dim3((unsigned)((Tk * Hk * D + 2047) / 2048), 2), dim3(256), 0, st, a);
