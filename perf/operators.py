@@ -316,7 +316,8 @@ def _norm_own(s):
         return [y, *torch.autograd.grad(y, (s["x"], s["w"]), s["dy"])]
     from casmtr_amd import ops
     if c["quant"]:
-        return [t for t in ops.rms_norm_quant(s["x"], s["w"], 1e-6, residual=s["res"], dtype=_F8[c["quant"]][0], group=c["group"] or None) if t is not None]
+        q, scale, h = ops.rms_norm_quant(s["x"], s["w"], 1e-6, residual=s["res"], dtype=_F8[c["quant"]][0], group=c["group"] or None)
+        return [t for t in (q, scale.view(c["rows"], -1), h) if t is not None]
     return [t for t in ops.rms_norm(s["x"], s["w"], 1e-6, residual=s["res"]) if t is not None]
 
 
