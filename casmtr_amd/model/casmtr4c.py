@@ -17,6 +17,7 @@ reference builds in every cross layer is never materialised (the matchers are bu
 data['stage_*']['idx_c01'].materialize() rebuilds it on request).
 """
 import math
+import os
 import threading
 
 import torch
@@ -231,6 +232,12 @@ class _ReducedAttention(nn.Module):
     def forward(self, x, H, W):
         B, N, C = x.shape
         nh = self.heads
+        if _fast(x) and C // nh <= 128 and os.environ.get("CASMTR_GLOBAL_ATTN") == "packed":   # own kernel, straight on the projections' outputs
+            r = _ln(self.norm, _tokens(_cv(self.sr, _grid(x, H, W))))
+            M = r.shape[1]
+            q, kv = _lin(self.q, x).reshape(B * N, nh, C // nh), self.kv(r).reshape(B * M, 2, nh, C // nh)
+            image = torch.arange(B + 1, device=x.device, dtype=torch.int32)
+            return _lin(self.proj, ops.packed_attn(q, kv[:, 0], kv[:, 1], image * N, image * M, scale=self.scale).reshape(B, N, C))
         q = _lin(self.q, x).reshape(B, N, nh, C // nh).permute(0, 2, 1, 3)
         r = _ln(self.norm, _tokens(_cv(self.sr, _grid(x, H, W))))
         kv = self.kv(r).reshape(B, -1, 2, nh, C // nh).permute(2, 0, 3, 1, 4)
