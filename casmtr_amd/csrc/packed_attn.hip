@@ -31,7 +31,7 @@ constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a m
 // FEW (few rows, long keys): a workgroup has 32 rows, its waves take 32 keys each of a tile and are joined in LDS at the end.  With 128 rows per
 // workgroup a tile takes each wave the whole way through 64 keys, for nothing where three of four waves have no rows of their own.
 template <typename T, int DP, int BN, int NW, bool DMA, bool FEW>
-__global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1 && DP <= 64)) ? 2 : 1) void packed_attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1 && DP <= 64)) ? (sizeof(T) == 2 && DP <= 64 ? 3 : 2) : 1) void packed_attn_kernel(const AttnArgs a) {
     typedef Tile<T, DP, BN> L;
     static_assert(!FEW || BN == 32 * NW, "one block of keys per wave");
     constexpr int BM = FEW ? 32 : 32 * NW, KS = DP / 16, NB = FEW ? 1 : BN / 32, DB = DP / 32;
@@ -104,12 +104,12 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
 #pragma unroll
                         for (int i = 0; i < 16; ++i) s[b][i] = seen_or(s[b][i], -INFINITY, 32 * b + 8 * (i >> 2) + (i & 3), lim);
                 }
-                float mx = s[0][0];
+                float big[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-                mx = max_halves(mx) * a.scale;
+                    for (int i = b ? 0 : 4; i < 16; ++i) big[i & 3] = fmaxf(big[i & 3], s[b][i]);
+                const float mx = max_halves(fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]))) * a.scale;
                 const bool up = mx > m + RESCALE_AT;   // (also the first tile: m = -inf); per row, so that a row's bits do not depend on its neighbours
                 if (__any(up)) {
                     const float f = !up ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
@@ -121,13 +121,15 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
                         for (int i = 0; i < 16; ++i) acc[d][i] *= f;
                 }
                 const float mm = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};   // four chains: one would wait for every addition
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.scale, -mm));
-                        l += s[b][i];
+                        sum[i & 3] += s[b][i];
                     }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll

@@ -54,7 +54,7 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&acc)[DB]) {
 
 // dq: a workgroup's rows are (token, head) pairs as in the forward kernel
 template <typename T, int DP, int BN, int NW, bool DMA>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <= 64) ? 2 : 1) void packed_attn_dq_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <= 64) ? (sizeof(T) == 2 && DP <= 64 ? 3 : 2) : 1) void packed_attn_dq_kernel(const BwdArgs a) {
     typedef Tile<T, DP, BN> L;
     constexpr int BM = 32 * NW, KS = DP / 16, NB = BN / 32, DB = DP / 32;
     __shared__ __attribute__((aligned(256))) char smem[TilePair<T, DP, BN, NW, DMA>::BYTES];
@@ -384,7 +384,7 @@ extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* 
         if (Tk > 0) {
             if (D <= 32) BWD_LAUNCH(packed_attn_dkv_kernel, E, 32, 64, qdma, kgrid);
             else if (D <= 64) BWD_LAUNCH(packed_attn_dkv_kernel, E, 64, (WIDE ? 32 : 64), qdma, kgrid);
-            else BWD_LAUNCH(packed_attn_dkv_kernel, T, 128, 32, qdma, kgrid);   // fp32 terms of K and V do not fit the registers here: 95 against 124 TFLOP/s
+            else BWD_LAUNCH(packed_attn_dkv_kernel, T, 128, (WIDE ? 32 : 64), qdma, kgrid);   // fp32 terms of K and V do not fit the registers here: 95 against 124 TFLOP/s
         }
 #undef BWD_LAUNCH
         if (splits > 1 && Tk > 0)
