@@ -3,7 +3,10 @@
 //   dq_i = sum_j ds_ij k_j;    dk_j = sum_i ds_ij q_i;    dv_j = sum_i p_ij do_i
 // No atomics: one kernel owns query rows and walks the keys (dq, and delta on the way), one owns keys and walks the query rows of all
 // heads that share them (dk, dv: the sum over the group is in the accumulator; in parts that a third kernel adds where there are few keys).  The scores are computed twice for it -- 7 products
-// instead of 5 -- and results repeat bit for bit.
+// instead of 5 -- and results repeat bit for bit.  Bound by the matrix instructions and, for heads of 64 and less, the exponentials beside them.
+// 16384 causal tokens, bf16: 32 / 8 heads of 128 dq 2.79 ms (1.18 PFLOP/s), dk and dv 5.03 ms (0.87; one wave per SIMD: K, V and both sums take 440
+// registers); 16 heads of 64 dq 0.78 ms (1.06), dk and dv 1.13 ms (0.98).
+// Roundings to 16 bits: p and ds, for the products with them (a probability below 2^-24 in fp16 is lost; it weighs nothing beside 2^-14).
 #include "packed_attn.hpp"
 
 using namespace casmtr;
@@ -330,11 +333,11 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(const BwdArgs
 constexpr int BWD_NW = 4;
 
 // Parts that the rows of a key tile are split into.  A key tile walks all rows of all the heads that share it, so few key heads leave the chip to
-// a few long workgroups (6 packed documents up to 4096, 4 key heads, 356 workgroups: 597 us with one part).  Each part costs a write
-// and a read of dk and dv in fp32.
+// a few long workgroups; each part costs a write and a read of dk and dv in fp32.  6 packed documents up to 4096, 4 key heads of 64, 372 key
+// tiles, both kernels with parts for at least 512 / 768 / 1024 / 1400 / 2048 workgroups: 346 / 339 / 307 / 327 / 316 us.
 int split_rows(long long Tk, int n, int Hk) {
     const long long wgs = slot_count(Tk, 1, n, 32 * BWD_NW) * Hk;
-    return wgs >= 2048 ? 1 : (int)(wgs >= 256 ? 1 + 2047 / wgs : 8);
+    return wgs >= 1024 ? 1 : (int)(wgs >= 128 ? 1 + 1023 / wgs : 8);
 }
 }  // namespace
 
