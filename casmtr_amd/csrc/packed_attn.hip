@@ -306,15 +306,19 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnArgs a)
 
 constexpr int FWD_NW = 4;
 
-// few rows: at most 32 (token, head of the group) rows per sequence on average
+// Few rows: at most 32 (token, head of the group) rows per sequence on average.  With 256 keys or more per sequence the waves of a workgroup share the
+// keys (FEW above); with fewer -- windows and the like, where neither four waves' rows nor four waves' keys are there -- a workgroup is one wave,
+// for heads of up to 64 (wider ones: the ordinary kernel).  8192 windows of 25 tokens, 8 heads of 16, bf16: one wave 174 us, FEW with four 547,
+// the ordinary kernel 435; 2048 x 32 rows x 128 keys, 8 heads of 128: 475, 637, 287.
 bool few_rows(long long Tq, int n, int H, int Hk) { return Tq * (H / Hk) <= 32LL * n; }
+bool long_keys(long long Tk, int n) { return Tk >= 256LL * n; }
 
 // How many parts a sequence's keys are split into: enough workgroups to fill the chip when there are few rows, and several times that many for few
 // rows, whose sequences may be of any length beside each other (16 single tokens against 161 to 32768 keys, 8 key heads of 128, bf16, up
 // to 512 / 1024 / 2048 / 4096 workgroups: 274 / 275 / 253 / 259 us; against 32768 each: 369 / 371 / 379 / 389 us, 5.8 to 5.5 TB/s).  A part is no shorter than 256 keys on average, so that what it writes (a
 // row of fp32 per query row) stays small beside what it reads.
 int split_count(long long Tq, long long Tk, int n, int H, int Hk) {
-    const bool few = few_rows(Tq, n, H, Hk);
+    const bool few = few_rows(Tq, n, H, Hk) && long_keys(Tk, n);
     const long long bm = few ? 32 : 32 * FWD_NW, tiles = (Tq * (H / Hk) + bm - 1) / bm, wgs = (tiles > n ? tiles : n) * Hk;
     if (wgs >= 512 && !few) return 1;
     long long s = (few ? 2048 : 1024) / (wgs > 0 ? wgs : 1);
@@ -335,13 +339,13 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
                                       long long kts, long long khs, long long vts, long long vhs, float scale, int causal, int dtype,
                                       casmtr_stream_t stream) {
     if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale < INFINITY) ||
-        Tq * (H / Hk) > 0x7fffffffLL || Tk > 0x7fffffffLL || Tq > 0x7fffffffLL)
+        Tq > 0x7fffff00LL || Tk > 0x7fffff00LL || Tq * (H / Hk) > 0x7fffff00LL)
         return CASMTR_ERR_UNSUPPORTED;
     if (Tq == 0) return 0;
     const int splits = split_count(Tq, Tk, nseq, H, Hk), G = H / Hk;
     if (splits > 1 && !ws) return CASMTR_ERR_UNSUPPORTED;
-    const bool few = few_rows(Tq, nseq, H, Hk);
-    const long long rows = Tq * H, wgs = slot_count(Tq, G, nseq, few ? 32 : 32 * FWD_NW) * Hk;
+    const bool few = few_rows(Tq, nseq, H, Hk) && long_keys(Tk, nseq), one = few_rows(Tq, nseq, H, Hk) && !few && D <= 64;
+    const long long rows = Tq * H, wgs = slot_count(Tq, G, nseq, few || one ? 32 : 32 * FWD_NW) * Hk;
     if (wgs > 0x7fffffffLL) return CASMTR_ERR_UNSUPPORTED;
     AttnArgs a{q, k, v, o, lse, ws, ws ? ws + (long long)splits * rows * D : nullptr, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk},
                qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits, scale * 1.44269504088896341f};
@@ -358,7 +362,10 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
         if (dma) hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, NW, true, FEW>), grid, dim3(64 * NW), 0, (hipStream_t)stream, a); \
         else hipLaunchKernelGGL((packed_attn_kernel<T, DP, BN, NW, false, FEW>), grid, dim3(64 * NW), 0, (hipStream_t)stream, a);    \
     } while (0)
-        if (few) {
+        if (one) {
+            if (D <= 32) FWD_LAUNCH(32, 32, 1, true);
+            else FWD_LAUNCH(64, 32, 1, true);
+        } else if (few) {
             if (D <= 32) FWD_LAUNCH(32, 128, 4, true);
             else if (D <= 64) FWD_LAUNCH(64, 128, 4, true);
             else FWD_LAUNCH(128, 64, 2, true);

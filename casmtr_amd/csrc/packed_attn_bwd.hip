@@ -352,7 +352,7 @@ extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* 
                                       int H, int Hk, int D, long long qts, long long qhs, long long kts, long long khs, long long vts, long long vhs,
                                       float scale, int causal, int dtype, casmtr_stream_t stream) {
     if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale < INFINITY) ||
-        Tq * (H / Hk) > 0x7fffffffLL || Tk > 0x7fffffffLL || Tq > 0x7fffffffLL || dtype < 0 || dtype > CASMTR_BF16)
+        Tq > 0x7fffff00LL || Tk > 0x7fffff00LL || Tq * (H / Hk) > 0x7fffff00LL || dtype < 0 || dtype > CASMTR_BF16)
         return CASMTR_ERR_UNSUPPORTED;
     if (Tq == 0 && Tk == 0) return 0;
     const int G = H / Hk;

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
     __shared__ float s_sum[TPR < 256 ? 1 : TPR / 64];
     __shared__ unsigned s_max[TPR < 256 ? 1 : TPR / 64];
     const int t = threadIdx.x % TPR;
-    const long long row = (long long)blockIdx.x * RPW + threadIdx.x / TPR;
+    const long long row = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RPW + threadIdx.x / TPR;
     if (row >= a.rows) return;   // whole waves only where a row is a wave's, the whole workgroup never otherwise
     const T* xr = (const T*)a.x + row * a.xs;
     const T* rr = a.res ? (const T*)a.res + row * a.rs : nullptr;
@@ -314,7 +314,9 @@ extern "C" int casmtr_rms_norm_fwd(const void* x, const void* residual, const vo
             typedef decltype(tv) T;
             ok = with_row_shape(C, [&](auto tpr, auto ch) {
                 constexpr int TPR = decltype(tpr)::value, CH = decltype(ch)::value, RPW = TPR < 256 ? 256 / TPR : 1;
-                hipLaunchKernelGGL((rms_norm_kernel<T, TPR, CH>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(TPR < 256 ? 256 : TPR), 0, (hipStream_t)stream, a);
+                const long long wgs = (rows + RPW - 1) / RPW, x = wgs < (1 << 21) ? wgs : 1 << 21;   // (a launch's x holds 2^32 threads)
+                hipLaunchKernelGGL((rms_norm_kernel<T, TPR, CH>), dim3((unsigned)x, (unsigned)((wgs + x - 1) / x)), dim3(TPR < 256 ? 256 : TPR), 0,
+                                   (hipStream_t)stream, a);
             });
         }) || !ok)
         return CASMTR_ERR_UNSUPPORTED;
