@@ -3,7 +3,7 @@
 PyTorch is plumbing here (device memory, streams); every computation below is a hand-written gfx950 kernel in
 libcasmtr_hip.so.  The preconditions mirror the reference's TORCH_CHECKs (score_computation.cpp:6-8): tensors must
 be device-resident and contiguous, fp32 values, int64 indices -- violations raise RuntimeError, nothing falls back
-to the CPU.
+to the CPU.  The operators on packed tokens (rms_norm, rotary, packed_attn) also take fp16 and bf16 and strided rows.
 """
 from __future__ import annotations
 
