@@ -48,15 +48,25 @@ __device__ __forceinline__ f32x16 mma(const frag_t<x3_t>& a, const frag_t<x3_t>&
     c = mma(a.t[0], b.t[1], c);
     return mma(a.t[0], b.t[0], c);
 }
+// eight values in three terms, two at a time: one conversion to a packed pair, whose halves are the pair's values in fp32 with a shift and a mask
+// (11 instructions per pair; from single conversions the compiler makes 15)
 __device__ __forceinline__ frag_t<x3_t> split3(const float (&x)[8]) {
-    frag_t<x3_t> f;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+    unsigned w[3][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        f.t[0][e] = (bf16_t)x[e];
-        const float r = x[e] - (float)f.t[0][e];
-        f.t[1][e] = (bf16_t)r;
-        f.t[2][e] = (bf16_t)(r - (float)f.t[1][e]);
+    for (int e = 0; e < 4; ++e) {
+        float u = x[2 * e], v = x[2 * e + 1];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            const bf16x2 p = __builtin_convertvector(f32x2{u, v}, bf16x2);
+            __builtin_memcpy(&w[j][e], &p, 4);
+            u -= __uint_as_float(w[j][e] << 16);
+            v -= __uint_as_float(w[j][e] & 0xffff0000u);
+        }
     }
+    frag_t<x3_t> f;
+    __builtin_memcpy(&f, w, sizeof(f));
     return f;
 }
 __device__ __forceinline__ f32x16 zero16() {
@@ -215,7 +225,7 @@ struct TileDma {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (unsigned)(64 * NW * i + 64 * wave) * 16u));
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff[i]), "s"(dst), "s"(rsrc) : "memory");
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff[i]), "s"(dst), "s"(rsrc) : "memory", "m0");
         }
     }
     // whether rows of this stride can be read so
