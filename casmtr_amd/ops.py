@@ -810,9 +810,9 @@ def rms_norm(x, weight, eps=1e-6, residual=None, want_rstd=False):
         h = round(x + residual);  y = h / sqrt(mean(h^2) + eps) * weight            (weight [C]: x's type or fp32)
     -> (y, h) -- h is the stream for the next residual, None without a residual --, with want_rstd (y, h, rstd fp32 [rows])."""
     R, C, xs, rs = _norm_args(x, weight, residual)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     h = torch.empty_like(y) if residual is not None else None
-    rstd = torch.empty(R, device=x.device, dtype=torch.float32) if want_rstd else None
+    rstd = x.new_empty(R, dtype=torch.float32) if want_rstd else None
     with _on(x.device):
         _lib.check(_lib.lib().casmtr_rms_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(y), _ptr(h), _ptr(rstd), None, R, C, xs, rs, float(eps),
                                                   _TOKEN_TYPES[x.dtype], _TOKEN_TYPES[weight.dtype], 0, 0, _stream()), "rms_norm_fwd")
@@ -829,9 +829,9 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn
     R, C, xs, rs = _norm_args(x, weight, residual)
     if group is not None and (group != 128 or C % 128):
         raise RuntimeError(f"rms_norm_quant: group must be None or 128 with C % 128 == 0, got group {group} and C {C}")
-    q = torch.empty(x.shape, device=x.device, dtype=dtype)
-    scale = torch.empty(x.shape[:-1] if group is None else (*x.shape[:-1], C // 128), device=x.device, dtype=torch.float32)
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
+    q = x.new_empty(x.shape, dtype=dtype)
+    scale = x.new_empty(x.shape[:-1] if group is None else (*x.shape[:-1], C // 128), dtype=torch.float32)
+    h = x.new_empty(x.shape) if residual is not None else None
     with _on(x.device):
         _lib.check(_lib.lib().casmtr_rms_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(q), _ptr(h), None, _ptr(scale), R, C, xs, rs, float(eps),
                                                   _TOKEN_TYPES[x.dtype], _TOKEN_TYPES[weight.dtype], _QUANT_TYPES[dtype], group or 0, _stream()),
@@ -842,20 +842,27 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn
 def rms_norm_bwd(dy, h, weight, rstd, dh=None):
     """Gradient of rms_norm: h [..., C] (x + residual as returned, or x), rstd from want_rstd, dh the gradient that reaches h from
     further on -> (dx [..., C], dweight [C]); dx is the gradient of x and of the residual.  The weight's sums have a fixed order."""
-    R, C, hs, _ = _norm_args(h, weight, None)
+    _norm_args(h, weight, None)
     _chk_tok(dy, "dy", h), _chk_tok(dh, "dh", h), _chk(rstd, "rstd")
-    if dy.shape != h.shape or (dh is not None and dh.shape != h.shape) or rstd.numel() != R or rstd.device != h.device:
+    if dy.shape != h.shape or (dh is not None and dh.shape != h.shape) or rstd.numel() * h.shape[-1] != h.numel() or rstd.device != h.device:
         raise RuntimeError("rms_norm_bwd: dy and dh must have h's shape, rstd one value per row")
-    dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    return _rms_norm_bwd(dy, h, weight, rstd, dh)
+
+
+def _rms_norm_bwd(dy, h, weight, rstd, dh):
+    """rms_norm_bwd of operands that are known to fit"""
+    R, C, hs = _rows(h, "h")
+    dx = h.new_empty(h.shape)
     if R == 0:
         return dx, torch.zeros_like(weight)
     dw = torch.empty_like(weight)
     l = _lib.lib()
-    ws = torch.empty(l.casmtr_rms_norm_bwd_ws_floats(R, C), device=h.device, dtype=torch.float32)
+    ws = h.new_empty(l.casmtr_rms_norm_bwd_ws_floats(R, C), dtype=torch.float32)
     with _on(h.device):
-        _lib.check(l.casmtr_rms_norm_bwd(_ptr(dy), _ptr(dh), _ptr(h), _ptr(weight), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws), R, C, _rows(dy, "dy")[2],
-                                         0 if dh is None else _rows(dh, "dh")[2], hs, _TOKEN_TYPES[h.dtype], _TOKEN_TYPES[weight.dtype], _stream()),
-                   "rms_norm_bwd")
+        rc = l.casmtr_rms_norm_bwd(dy.data_ptr(), _ptr(dh), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(),
+                                   R, C, _rows(dy, "dy")[2], 0 if dh is None else _rows(dh, "dh")[2], hs, _TOKEN_TYPES[h.dtype],
+                                   _TOKEN_TYPES[weight.dtype], _stream())
+    _lib.check(rc, "rms_norm_bwd")
     return dx, dw
 
 
@@ -918,8 +925,8 @@ def rotary(q, k, positions, inv_freq, layout="half", gain=1.0, inverse=False):
         raise RuntimeError("rotary: positions must be [T] or [T,2] and inv_freq a vector, on q's device")
     if n < 1 or 2 * n > D or n > 1024 or (axes == 2 and n % 2):
         raise RuntimeError(f"rotary: 1 to min(D / 2, 1024) pairs (an even number with two positions per token), got {n} for D {D}")
-    oq = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
-    ok = torch.empty((T, Hk, D), device=q.device, dtype=q.dtype) if k is not None else None
+    oq = q.new_empty((T, Hq, D))
+    ok = q.new_empty((T, Hk, D)) if k is not None else None
     with _on(q.device):
         _lib.check(_lib.lib().casmtr_rotary_fwd(_ptr(q), _ptr(k), _ptr(positions), _ptr(inv_freq), _ptr(oq), _ptr(ok), T, Hq, Hk, D, n, axes,
                                                 int(positions.dtype == torch.int64), int(layout == "interleaved"), float(gain), int(bool(inverse)),
@@ -965,11 +972,11 @@ def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, 
     synchronisation; safe to capture into a HIP graph."""
     cu_k, scale, sizes, strides = _packed_args(q, k, v, cu_q, cu_k, len_k, scale)
     dev, dt = q.device, q.dtype
-    out = torch.empty(q.shape, device=dev, dtype=dt)
-    lse = torch.empty(q.shape[:2], device=dev, dtype=torch.float32) if want_lse else None
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if want_lse else None
     l = _lib.lib()
     wsf = l.casmtr_packed_attn_ws_floats(*sizes)
-    ws = torch.empty(wsf, device=dev, dtype=torch.float32) if wsf else None
+    ws = q.new_empty(wsf, dtype=torch.float32) if wsf else None
     with _on(dev):
         rc = l.casmtr_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(ws), cu_q.data_ptr(), cu_k.data_ptr(),
                                       _ptr(len_k), *sizes, *strides, scale, 1 if causal else 0, _TOKEN_TYPES[dt], _stream())
@@ -985,13 +992,18 @@ def packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k=None, len_k=None, causal
     for t, name, shape, dtype in ((grad, "grad", (Tq, H, D), q.dtype), (out, "out", (Tq, H, D), q.dtype), (lse, "lse", (Tq, H), torch.float32)):
         if tuple(_chk(t, name, dtype).shape) != shape or t.device != q.device:
             raise RuntimeError(f"packed_attn_bwd: {name} must be {shape} on {q.device}")
-    dq = torch.empty((Tq, H, D), device=q.device, dtype=q.dtype)
-    dk, dv = (torch.empty((Tk, Hk, D), device=q.device, dtype=q.dtype) for _ in range(2))
+    return _packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k, len_k, causal, scale, sizes, strides)
+
+
+def _packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k, len_k, causal, scale, sizes, strides):
+    """packed_attn_bwd of operands that are known to fit (sizes, strides: as _packed_args gives them)"""
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     l = _lib.lib()
     wsf = l.casmtr_packed_attn_bwd_ws_floats(*sizes)
-    ws = torch.empty(wsf, device=q.device, dtype=torch.float32) if wsf else None
+    ws = q.new_empty(wsf, dtype=torch.float32) if wsf else None
     with _on(q.device):
-        _lib.check(l.casmtr_packed_attn_bwd(_ptr(grad), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), _ptr(cu_q),
-                                            _ptr(cu_k), _ptr(len_k), *sizes, *strides, scale, int(bool(causal)), _TOKEN_TYPES[q.dtype], _stream()),
-                   "packed_attn_bwd")
+        rc = l.casmtr_packed_attn_bwd(grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                      dv.data_ptr(), _ptr(ws), cu_q.data_ptr(), cu_k.data_ptr(), _ptr(len_k), *sizes, *strides, scale,
+                                      1 if causal else 0, _TOKEN_TYPES[q.dtype], _stream())
+    _lib.check(rc, "packed_attn_bwd")
     return dq, dk, dv
