@@ -3,7 +3,7 @@
 // Row i of a sequence with nq rows and nk keys sees all keys, or, causal, the keys j <= i + nk - nq.  A row that sees none gives 0 and -inf.
 // Query heads share key heads in groups of G = H / Hk.
 //
-// fp32 runs as three bf16 terms (x3_t) -- 8 x 43264 rows x 676 keys, 4 heads of 32: 825 us (145 TFLOP/s) against 1118 us on the fp32 matrix
+// fp32 runs as three bf16 terms (x3_t) -- 8 x 43264 rows x 676 keys, 4 heads of 32: 0.76 to 0.80 ms (150 TFLOP/s and more) against 1.12 ms on the fp32 matrix
 // instructions, whose 154 TFLOP/s bound it --, except for few rows, where the reads bound it.
 //
 // One pass over the keys with the running maximum and sum of the softmax.  A tile's rows are (token, head of the group) pairs, token-major, so
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
 #pragma unroll
                     for (int st = 0; st < KS; ++st) {
                         const frag_t<T> kf = L::rows(ks, wkey + 32 * b + r, st, h);
-                        s[b] = GUARD ? mma_any<T>(kf, qf[st], s[b]) : mma(kf, qf[st], s[b]);
+                        s[b] = GUARD ? mma_any<T>(kf, qf[st], s[b], h) : mma(kf, qf[st], s[b]);
                     }
                 }
                 if (hidden) {

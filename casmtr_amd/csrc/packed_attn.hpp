@@ -419,15 +419,16 @@ __device__ __forceinline__ f32x16 mma_hidden(const frag_t<T>& a, const frag_t<T>
     }
     return c;
 }
-// c += A B as the formula has it where either holds infinities or NaN.  Of three terms the second and third of an infinity are NaN: such
-// elements are multiplied by their first term alone.
+// c += A B as the formula has it where either holds infinities or NaN.  Of three terms the second and third of an infinity are NaN: such elements
+// are left out of the product of terms (so that the other pairs keep its bits), and an index that has any is multiplied by itself, first
+// terms only: what is not finite then is what the left-out elements add.
 template <typename T>
-__device__ __forceinline__ f32x16 mma_any(const frag_t<T>& a, const frag_t<T>& b, f32x16 c) {
+__device__ __forceinline__ f32x16 mma_any(const frag_t<T>& a, const frag_t<T>& b, f32x16 c, int h) {
     if constexpr (!std::is_same<T, x3_t>::value) return mma(a, b, c);
     else {
         if (!any_not_finite<bf16_t>(a.t[0]) && !any_not_finite<bf16_t>(b.t[0])) return mma(a, b, c);
         frag_t<x3_t> fa, fb;
-        frag_t<bf16_t> oa, ob;
+        unsigned odd = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool ka = __builtin_fabsf((float)a.t[0][e]) < INFINITY, kb = __builtin_fabsf((float)b.t[0][e]) < INFINITY;
@@ -436,12 +437,24 @@ __device__ __forceinline__ f32x16 mma_any(const frag_t<T>& a, const frag_t<T>& b
                 fa.t[j][e] = ka ? a.t[j][e] : (bf16_t)0.f;
                 fb.t[j][e] = kb ? b.t[j][e] : (bf16_t)0.f;
             }
-            oa[e] = ka ? (bf16_t)0.f : a.t[0][e];
-            ob[e] = kb ? (bf16_t)0.f : b.t[0][e];
+            odd |= (ka && kb ? 0u : 1u) << (8 * h + e);
         }
         c = mma(fa, fb, c);
-        c = mma(oa, b.t[0], c);
-        return mma(fa.t[0], ob, c);
+        for (int n = 0; n < 16; ++n) {
+            if (!__any((odd >> n) & 1u)) continue;
+            frag_t<bf16_t> a1, b1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool on = n == 8 * h + e;
+                a1[e] = on ? a.t[0][e] : (bf16_t)0.f;
+                b1[e] = on ? b.t[0][e] : (bf16_t)0.f;
+            }
+            const f32x16 d = mma(a1, b1, zero16());
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!(__builtin_fabsf(d[i]) < INFINITY)) c[i] += d[i];
+        }
+        return c;
     }
 }
 

@@ -120,8 +120,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <=
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
                     const frag_t<T> kf = L::rows(ks, 32 * b + r, st, h), vf = L::rows(vs, 32 * b + r, st, h);
-                    s = GUARD ? mma_any<T>(kf, qf[st], s) : mma(kf, qf[st], s);
-                    dp = GUARD ? mma_any<T>(vf, gf[st], dp) : mma(vf, gf[st], dp);
+                    s = GUARD ? mma_any<T>(kf, qf[st], s, h) : mma(kf, qf[st], s);
+                    dp = GUARD ? mma_any<T>(vf, gf[st], dp, h) : mma(vf, gf[st], dp);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
         const int hd = hk * G + n / per, t = t0 + n % per;
         if (tid < BM) {
             const int tok = t * BM + tid;
-            sl = INFINITY;   // a row that is not there or sees nothing: its probabilities are exactly 0
+            sl = INFINITY;   // a row that sees nothing: its probabilities are exactly 0
             sd = 0.f;
             if (tok < rows.count) {
                 const long long at = (long long)(rows.begin + tok) * a.H + hd;
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
             __syncthreads();
             if (n + 1 < turns) fetch(n + 1, stage ^ 1);
             if ((t + 1) * BM <= wave_first) return;
-            const bool hidden = t * BM < wave_all;
+            const bool hidden = t * BM < wave_all || (t + 1) * BM > rows.count;   // (zeros stand for rows behind the last: 0 * inf)
             const char *qs = qg.first(stage), *gs = qg.second(stage);
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
@@ -239,8 +239,8 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
                     const frag_t<T> qf = L::rows(qs, 32 * b + r, st, h), gf = L::rows(gs, 32 * b + r, st, h);
-                    s = GUARD ? mma_any<T>(qf, kf[st], s) : mma(qf, kf[st], s);
-                    dp = GUARD ? mma_any<T>(gf, vf[st], dp) : mma(gf, vf[st], dp);
+                    s = GUARD ? mma_any<T>(qf, kf[st], s, h) : mma(qf, kf[st], s);
+                    dp = GUARD ? mma_any<T>(gf, vf[st], dp, h) : mma(gf, vf[st], dp);
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
@@ -256,12 +256,12 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
                 // element n & 7 of half n >> 3 of step tt stands for token t BM + 32 b + 16 tt + 8 (n >> 2 & 1) + 4 (n >> 3) + (n & 3)
                 const int tok0 = t * BM + 32 * b;
                 if (hidden) {
-                    const int lo = first - tok0 - 4 * h;   // (rows behind the last are excluded by their lse)
+                    const int lo = first - tok0 - 4 * h, hi = rows.count - tok0 - 4 * h;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int x = 8 * (i >> 2) + (i & 3);
-                        s[i] = seen_or(s[i], 0.f, -1 - x, -lo);
-                        dp[i] = seen_or(dp[i], 0.f, -1 - x, -lo);
+                        s[i] = seen_or(seen_or(s[i], 0.f, -1 - x, -lo), 0.f, x, hi);
+                        dp[i] = seen_or(seen_or(dp[i], 0.f, -1 - x, -lo), 0.f, x, hi);
                     }
                 }
 #pragma unroll

@@ -297,6 +297,28 @@ def test_hidden_infinities(H, Hk, D, dt):
             assert out[220:240].isnan().all()
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (3, 1, 128), (2, 2, 32)])
+def test_key_of_no_weight(H, Hk, D, dt):
+    """a key whose scores are -inf weighs nothing: the outputs are those without it, its own gradients are 0 (row counts beside the tiles')"""
+    from casmtr_amd import ops
+    for lens in ([(70, 50)], [(33, 90), (5, 21)]):
+        q, k, v, cq, ck = make(lens, H, Hk, D, dt, tail=0)
+        q[..., 0] = q[..., 0].abs() + 0.1
+        g = torch.randn(q.shape, device="cuda").to(dt)
+        k2 = k.clone()
+        k2[20, :, 0] = -math.inf
+        out, lse = ops.packed_attn(q, k2, v, cq, ck, want_lse=True)
+        _, dk, dv = ops.packed_attn_bwd(g, q, k2, v, out, lse, cq, ck)
+        less = [(lens[0][0], lens[0][1] - 1)] + lens[1:]
+        keep = torch.arange(k.shape[0], device="cuda") != 20
+        check(out, lse, reference(q, k[keep], v[keep], less, False, D ** -0.5))
+        assert (dk[20] == 0).all() and (dv[20] == 0).all()
+        otol = reference(q, k[keep], v[keep], less, False, D ** -0.5)[1]
+        _, (rk, tk), (rv, tv) = reference_grads(g, q, k[keep], v[keep], less, False, D ** -0.5, otol)
+        assert ((dk[keep].double() - rk).abs() <= tk).all() and ((dv[keep].double() - rv).abs() <= tv).all()
+
+
 def test_wrong_lengths_stay_inside():
     """arrays that claim more than there is: nothing outside the tensors is read or written (what the rows hold is not defined)"""
     from casmtr_amd import ops
