@@ -13,15 +13,15 @@ class PackedAttention(Function):
     def forward(ctx, q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
         out, lse = ops.packed_attn(q, k, v, cu_q, cu_k, len_k, causal, scale, want_lse=True)
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, len_k)
-        ctx.args = causal, ops._packed_args(q, k, v, cu_q, cu_k, len_k, scale)
+        ctx.args = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         q, k, v, out, lse, cu_q, cu_k, len_k = ctx.saved_tensors
-        causal, (_, scale, sizes, strides) = ctx.args   # (checked by the forward pass)
-        dq, dk, dv = ops._packed_attn_bwd(grad.contiguous(), q, k, v, out, lse, cu_q, cu_q if cu_k is None else cu_k, len_k, causal, scale, sizes, strides)
+        # everything about the operands is taken from the tensors as they are NOW: hooks (offloading, compression) may give back other strides
+        dq, dk, dv = ops.packed_attn_bwd(grad.contiguous(), q, k, v, out, lse, cu_q, cu_k, len_k, *ctx.args)
         return dq, dk, dv, None, None, None, None, None
 
 

@@ -992,11 +992,6 @@ def packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k=None, len_k=None, causal
     for t, name, shape, dtype in ((grad, "grad", (Tq, H, D), q.dtype), (out, "out", (Tq, H, D), q.dtype), (lse, "lse", (Tq, H), torch.float32)):
         if tuple(_chk(t, name, dtype).shape) != shape or t.device != q.device:
             raise RuntimeError(f"packed_attn_bwd: {name} must be {shape} on {q.device}")
-    return _packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k, len_k, causal, scale, sizes, strides)
-
-
-def _packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k, len_k, causal, scale, sizes, strides):
-    """packed_attn_bwd of operands that are known to fit (sizes, strides: as _packed_args gives them)"""
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     l = _lib.lib()
     wsf = l.casmtr_packed_attn_bwd_ws_floats(*sizes)
