@@ -842,16 +842,10 @@ def rms_norm_quant(x, weight, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn
 def rms_norm_bwd(dy, h, weight, rstd, dh=None):
     """Gradient of rms_norm: h [..., C] (x + residual as returned, or x), rstd from want_rstd, dh the gradient that reaches h from
     further on -> (dx [..., C], dweight [C]); dx is the gradient of x and of the residual.  The weight's sums have a fixed order."""
-    _norm_args(h, weight, None)
+    R, C, hs, _ = _norm_args(h, weight, None)
     _chk_tok(dy, "dy", h), _chk_tok(dh, "dh", h), _chk(rstd, "rstd")
     if dy.shape != h.shape or (dh is not None and dh.shape != h.shape) or rstd.numel() * h.shape[-1] != h.numel() or rstd.device != h.device:
         raise RuntimeError("rms_norm_bwd: dy and dh must have h's shape, rstd one value per row")
-    return _rms_norm_bwd(dy, h, weight, rstd, dh)
-
-
-def _rms_norm_bwd(dy, h, weight, rstd, dh):
-    """rms_norm_bwd of operands that are known to fit"""
-    R, C, hs = _rows(h, "h")
     dx = h.new_empty(h.shape)
     if R == 0:
         return dx, torch.zeros_like(weight)

@@ -86,6 +86,19 @@ def test_attention_refuses_changed_tensors(stub, change):
     assert "casmtr_packed_attn_bwd" not in stub.calls
 
 
+@pytest.mark.parametrize("change", [lambda t: t.float() if t.dtype == torch.bfloat16 and t.dim() == 2 else t, lambda t: t[:-1] if t.dim() == 2 else t,
+                                    lambda t: t.half() if t.dtype == torch.float32 else t])
+def test_norm_refuses_changed_tensors(stub, change):
+    from casmtr_amd.functions.rms_norm import rms_norm_op
+    x, w = torch.randn(6, 32).bfloat16().requires_grad_(), torch.ones(32).bfloat16().requires_grad_()
+    ctx, _ = _hooked(change)
+    with ctx:
+        y = rms_norm_op(x, w)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    assert "casmtr_rms_norm_bwd" not in stub.calls
+
+
 def test_norm_strides_follow_the_saved_tensors(stub):
     from casmtr_amd.functions.rms_norm import rms_norm_op
     wide = torch.randn(6, 50).requires_grad_()
