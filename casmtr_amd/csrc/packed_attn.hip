@@ -191,8 +191,9 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
 #pragma unroll
             for (int j = 0; j < NW; ++j) {
                 const float mj = stat[j * 32 + rr], lj = stat[(NW + j) * 32 + rr];
+                // m of -inf: the wave saw no key (its sums are zeros) or none of weight.  A share is added whatever its weight: where that underflows, an
+                // infinity or NaN in it still reaches the row, as it does where one wave walks all keys (0 * inf)
                 w[j] = mj == -INFINITY ? (lj != lj ? lj : 0.f) : __builtin_amdgcn_exp2f(mj - M);
-                if (w[j] == 0.f) continue;   // a wave that saw no key
                 const f32x4 x = *reinterpret_cast<const f32x4*>(share + (j * 32 + rr) * LD + c);
                 ls += w[j] * lj;
 #pragma unroll
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnArgs a)
         ls = ml[1];
     }
     const float m = wave_max_f32(ms);
-    const float w = ms == -INFINITY ? (ls != ls ? ls : 0.f) : __builtin_amdgcn_exp2f(ms - m);   // 0: a split that sees no key
+    const float w = ms == -INFINITY ? (ls != ls ? ls : 0.f) : __builtin_amdgcn_exp2f(ms - m);
     float l = 0.f, o0 = 0.f, o1 = 0.f;
     const float* po = a.part_o + row * a.D;
     for (int s = 0; s < a.splits; s += 4) {   // four splits' loads in flight
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnArgs a)
         for (int j = 0; j < 4; ++j) {
             const float f = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(w), min(s + j, 63)));
             const float lj = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(ls), min(s + j, 63)));
-            if (s + j >= a.splits || f == 0.f) continue;
+            if (s + j >= a.splits) continue;   // (weights of 0 are added too: see the join of the waves above)
             l += f * lj;
             o0 += f * x0[j];
             o1 += f * x1[j];

@@ -1,0 +1,47 @@
+"""Packed attention at the edges of its numbers: shares of the keys whose weight underflows, probabilities and score gradients below fp16's
+normal range, fp32 magnitudes next to the largest."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def cu(lens):
+    t = torch.zeros(len(lens) + 1, dtype=torch.int32)
+    t[1:] = torch.tensor(lens).cumsum(0)
+    return t.cuda()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 128), (4, 4, 32), (4, 2, 64)])
+@pytest.mark.parametrize("rows,keys", [(1, 4096), (5, 700), (1, 300), (40, 3000), (300, 3000), (5, 100)])
+@pytest.mark.parametrize("at", [2, -1])
+def test_visible_infinities_in_shares_of_no_weight(at, rows, keys, H, Hk, D, dt):
+    """One key's score lies 400 above all others, so whatever part of the keys it is not in weighs exp(-400) = 0 beside it.  An infinity or NaN
+    at a visible key of such a part reaches the row all the same (0 * inf), however the keys are split, and no other row or column."""
+    from casmtr_amd import ops
+    g = torch.Generator().manual_seed(keys)
+    q, k, v = (0.1 * torch.randn(n, h, D, generator=g) for n, h in ((2 * rows, H), (2 * keys, Hk), (2 * keys, Hk)))
+    q[..., 0], k[..., 0] = 20.0, 0.0
+    top = -1 if at == 2 else 2           # of each sequence
+    for s in (0, 1):
+        k[s * keys + top % keys, :, 0] = 20.0
+    q, k, v = (t.to(dt).cuda() for t in (q, k, v))
+    cq, ck = cu([rows] * 2), cu([keys] * 2)
+    clean, lse = ops.packed_attn(q, k, v, cq, ck, scale=1.0, want_lse=True)
+    assert clean.isfinite().all() and (lse >= 390).all()
+    cols = torch.arange(D, device="cuda") != 5
+    for bad in (math.nan, math.inf):
+        v2 = v.clone()
+        v2[at % keys, :, 5] = bad        # the first sequence alone
+        out, l2 = ops.packed_attn(q, k, v2, cq, ck, scale=1.0, want_lse=True)
+        assert not out[:rows, :, 5].isfinite().any()
+        assert torch.equal(out[:rows][..., cols], clean[:rows][..., cols]) and torch.equal(out[rows:], clean[rows:]) and torch.equal(l2, lse)
+    k2 = k.clone()
+    k2[at % keys, :, 3] = math.nan       # a score that is not a number
+    out, l2 = ops.packed_attn(q, k2, v, cq, ck, scale=1.0, want_lse=True)
+    assert out[:rows].isnan().all() and l2[:rows].isnan().all()
+    assert torch.equal(out[rows:], clean[rows:]) and torch.equal(l2[rows:], lse[rows:])
