@@ -31,6 +31,10 @@ struct AttnArgs {
 
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a maximum grew by more than 8 bits: exp2 stays below 256, far from any overflow
+// Probabilities are multiplied as 2^P_BITS of their value: in fp16 they stay in the normal range down to 2^-21 of the row's largest then, and what is lost
+// below that is at most 2^-32 of it each -- beside 2^-25 without, which 65536 keys of 2^-25 make up to a whole result.  2^(RESCALE_AT + 7) is within
+// fp16.  The row's sum carries the same factor, so only lse has to take it out.
+template <typename T> constexpr float P_BITS = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 
 // FEW (few rows, long keys): a workgroup has 32 rows, its waves take 32 keys each of a tile and are joined in LDS at the end.  With 128 rows per
 // workgroup a tile takes each wave the whole way through 64 keys, for nothing where three of four waves have no rows of their own.
@@ -124,7 +128,7 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
 #pragma unroll
                         for (int i = 0; i < 16; ++i) acc[d][i] *= f;
                 }
-                const float mm = m == -INFINITY ? 0.f : m;
+                const float mm = m == -INFINITY ? 0.f : m - P_BITS<T>;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};   // four chains: one would wait for every addition
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -138,7 +142,7 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int tt = 0; tt < 2; ++tt) {
-                        const frag_t<T> p = to_frag<T>(s[b], tt);   // probabilities below 256 rounded to the values' type; l sums the unrounded ones
+                        const frag_t<T> p = to_frag<T>(s[b], tt);   // probabilities below 256 (2^15 with P_BITS) rounded to the values' type; l sums the unrounded ones
                         const int k0 = 32 * b + 16 * tt;
 #pragma unroll
                         for (int d = 0; d < DB; ++d) {
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (c + e < a.D) orow[c + e] = (store_t<T>)(o[e] * inv);
-            if (a.lse && c == 0) a.lse[at] = some ? (M + __builtin_amdgcn_logf(ls)) * LN2 : -INFINITY;
+            if (a.lse && c == 0) a.lse[at] = some ? (M - P_BITS<T> + __builtin_amdgcn_logf(ls)) * LN2 : -INFINITY;
         }
         return;
     }
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
                 for (int e = 0; e < 4; ++e)
                     if (c + e < a.D) orow[c + e] = v[e];
         }
-    if (a.lse && h == 0) a.lse[out_row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    if (a.lse && h == 0) a.lse[out_row] = l > 0.f || l != l ? (m - P_BITS<T> + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 // joins the splits of a row: weights 2^(m_s - max m); one wave per row, lane s holds the weight of split s (at most 64)
@@ -302,7 +306,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnArgs a)
     T* orow = (T*)a.o + row * a.D;
     if (lane < a.D) orow[lane] = (T)(o0 * inv);
     if (lane + 64 < a.D) orow[lane + 64] = (T)(o1 * inv);
-    if (a.lse && lane == 0) a.lse[row] = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    if (a.lse && lane == 0) a.lse[row] = some ? (m - P_BITS<T> + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 constexpr int FWD_NW = 4;

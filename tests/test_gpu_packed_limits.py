@@ -45,3 +45,30 @@ def test_visible_infinities_in_shares_of_no_weight(at, rows, keys, H, Hk, D, dt)
     out, l2 = ops.packed_attn(q, k2, v, cq, ck, scale=1.0, want_lse=True)
     assert out[:rows].isnan().all() and l2[:rows].isnan().all()
     assert torch.equal(out[rows:], clean[rows:]) and torch.equal(l2[rows:], lse[rows:])
+
+
+# ---- fp16: what lies below its normal range.  u = 2^-24.  A probability is rounded at 2^7 times its value relative to the row's maximum: half a step of fp16 of
+# itself (2^-11), and below the normal range half a subnormal step, 2^-25, of that: 2^-32 of the row's sum.
+U = 2.0 ** -24
+H16 = 2.0 ** -11
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("rows,keys", [(1, 65536), (40, 20000), (200, 8192), (3, 200)])
+def test_fp16_many_small_probabilities(rows, keys, D):
+    """one key takes nearly all the weight and has a value of 0; the others weigh 2^-17 to 2^-25 of it each and make up the result together"""
+    from casmtr_amd import ops
+    for bits in (17.0, 21.5, 24.75):
+        q, k = torch.zeros(rows, 1, D), torch.zeros(keys, 1, D)
+        q[..., 0], k[1:, :, 0] = 1.0, -bits * math.log(2)
+        v = torch.rand(keys, 1, D, generator=torch.Generator().manual_seed(D)) + 0.5
+        v[0] = 0
+        q, k, v = (t.half().cuda() for t in (q, k, v))
+        for top in (0, keys - 1):
+            k[[0, top]], v[[0, top]] = k[[top, 0]], v[[top, 0]]
+            out = ops.packed_attn(q, k, v, cu([rows]), cu([keys]), scale=1.0)
+            p = torch.softmax(q[:, 0].double() @ k[:, 0].double().t(), 1)
+            ref = p @ v[:, 0].double()
+            es = ((D + 8) * U * (q[:, 0].abs().double() @ k[:, 0].abs().double().t()) * 2).amax()
+            tol = (2 * H16 + 2 * es + (keys + 32) * U) * ref + keys * 2.0 ** -32 * 1.5 + 2.0 ** -25
+            assert ((out[:, 0].double() - ref).abs() <= tol).all(), ((out[:, 0].double() - ref).abs() / tol).max().item()
