@@ -6,7 +6,9 @@
 // instead of 5 -- and results repeat bit for bit.  Bound by the matrix instructions and, for heads of 64 and less, the exponentials beside them.
 // 16384 causal tokens, bf16: 32 / 8 heads of 128 dq 2.79 ms (1.18 PFLOP/s), dk and dv 5.03 ms (0.87; one wave per SIMD: K, V and both sums take 440
 // registers); 16 heads of 64 dq 0.78 ms (1.06), dk and dv 1.13 ms (0.98).
-// Roundings to 16 bits: p and ds, for the products with them (a probability below 2^-24 in fp16 is lost; it weighs nothing beside 2^-14).
+// Roundings to 16 bits: p and ds, for the products with them.  In fp16 at a power of two that keeps them in its normal range: p (at most 1, the smaller
+// the more keys there are) at 2^12, ds, whose size follows the gradient's, at a running one (in_range).  Unscaled, gradients of 1e-3 over
+// 4096 keys lost most of their bits on the way to dq and dk.
 #include "packed_attn.hpp"
 
 using namespace casmtr;
@@ -43,6 +45,42 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], int h
                 for (int e = 0; e < 4; ++e)
                     if (c + e < D) row[c + e] = v[e];
         }
+}
+
+// bits by which p is raised for the product with do.  Not all 15 that there are: lse is rounded, and where scores are so large that this shows, p may
+// come out somewhat above 1.
+template <typename T> constexpr float P_BITS = std::is_same<T, f16_t>::value ? 12.f : 0.f;
+// fp16: x (32 contraction indices of this lane's column) times 2^e, where e brings the column's largest |x| so far to 2^8 at least and below 2^15; when one
+// comes that passes that, e is lowered and the sums so far follow, which is exact.  What is rounded below the normal range then loses at most
+// 2^-33 of the largest.  (e starts at 127, where the first |x| of 2^-112 or more lowers it.)  Infinities and NaN stay what they are.
+constexpr int E_START = 127;
+template <typename T, int DB>
+__device__ __forceinline__ void in_range(f32x16& x, f32x16 (&sum)[DB], int& e) {
+    if constexpr (std::is_same<T, f16_t>::value) {
+        float big[4] = {__builtin_fabsf(x[0]), __builtin_fabsf(x[1]), __builtin_fabsf(x[2]), __builtin_fabsf(x[3])};
+#pragma unroll
+        for (int i = 4; i < 16; ++i) big[i & 3] = fmaxf(big[i & 3], __builtin_fabsf(x[i]));
+        const float mx = max_halves(fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])));   // (both halves hold parts of the column's sum)
+        const int ex = (int)((__float_as_uint(mx) >> 23) & 255u) - 127;                      // -127 (zero) .. 128 (infinity)
+        const bool up = ex + e > 14;
+        if (__any(up)) {
+            const int lower = up ? 8 - ex - e : 0;
+            e += lower;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[d][i] = __builtin_amdgcn_ldexpf(sum[d][i], lower);
+        }
+        const float f = __uint_as_float((unsigned)(e + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= f;
+    }
+}
+// the factor that takes 2^e and `bits` out of such a sum again
+template <typename T>
+__device__ __forceinline__ float out_of_range(float f, int e, float bits = 0.f) {
+    if constexpr (std::is_same<T, f16_t>::value) return __builtin_amdgcn_ldexpf(f, -e - (int)bits);
+    else return f;
 }
 
 template <int DB>
@@ -98,11 +136,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <=
     const float lse = a.lse[out_row], lse2 = lse == -INFINITY ? 0.f : lse * LOG2E;   // (a row that sees nothing: every key is hidden below)
     if (h == 0 && row < nrow) a.delta[out_row] = delta;
     f32x16 acc[DB];
+    int e = E_START;
     TilePair<T, DP, BN, NW, DMA> kv;
     kv.init(smem, tid, wave, a.kts, a.vts, a.D);
     kv.of((const store_t<T>*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const store_t<T>*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
     const auto pass = [&](auto guard) {
         constexpr bool GUARD = decltype(guard)::value;
+        e = E_START;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         if (0 < t1) kv.fetch(0, 0);
@@ -133,6 +173,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <=
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = seen_or(s[i], 0.f, 32 * b + 8 * (i >> 2) + (i & 3), lim);
                 }
+                in_range<T, DB>(s, acc, e);
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
                     const frag_t<T> ds = to_frag<T>(s, tt);   // rounded to the keys' type for the product with them
@@ -155,7 +196,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <=
     if (a.s.causal || std::is_same<T, x3_t>::value) {   // as in the forward kernel: a sum that is not finite may have met a hidden infinity
         if (__syncthreads_or(not_finite(acc))) pass(std::true_type{});
     }
-    if (row < nrow) store_row<store_t<T>, DB>((store_t<T>*)a.dq + out_row * a.D, acc, h, a.D, a.scale);
+    if (row < nrow) store_row<store_t<T>, DB>((store_t<T>*)a.dq + out_row * a.D, acc, h, a.D, out_of_range<T>(a.scale, e));
 }
 
 // dk, dv: a workgroup owns BN = 32 NW keys of one key head, a wave 32 of them (K and V stay in its registers), and walks the rows of the heads that
@@ -192,6 +233,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
         }
     }
     f32x16 dk[DB], dv[DB];
+    int e = E_START;
     const int t0 = wg_first / BM, per = (rows.count + BM - 1) / BM - t0;   // tiles of a head
     int n0 = 0, turns = wg_first < rows.count ? per * G : 0;                // of all heads, of this split
     if (a.splits > 1) {
@@ -211,7 +253,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
             if (tok < rows.count) {
                 const long long at = (long long)(rows.begin + tok) * a.H + hd;
                 const float x = a.lse[at];
-                sl = x == -INFINITY ? INFINITY : x * LOG2E;
+                sl = x == -INFINITY ? INFINITY : x * LOG2E - P_BITS<T>;
                 sd = a.delta[at];
             }
         }
@@ -222,6 +264,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
         constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
         for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+        e = E_START;
         if (n0 < turns) fetch(n0, 0);
         const auto step = [&](int n, auto stage_) {
             constexpr int stage = decltype(stage_)::value;
@@ -264,6 +307,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
                         dp[i] = seen_or(seen_or(dp[i], 0.f, -1 - x, -lo), 0.f, x, hi);
                     }
                 }
+                in_range<T, DB>(dp, dk, e);
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
                     const frag_t<T> pf = to_frag<T>(s, tt), df = to_frag<T>(dp, tt);   // rounded to the rows' type for the products with them
@@ -302,15 +346,16 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
 #pragma unroll
         for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     }
+    const float fk = out_of_range<T>(a.scale, e, P_BITS<T>), fv = out_of_range<T>(1.f, 0, P_BITS<T>);
     if (a.splits > 1) {
         const long long n = a.s.Tk * a.Hk * a.D;
         float* part = a.part + 2 * n * blockIdx.y + out_row * a.D;
-        store_row<float, DB>(part, dk, h, a.D, a.scale);
-        store_row<float, DB>(part + n, dv, h, a.D, 1.f);
+        store_row<float, DB>(part, dk, h, a.D, fk);
+        store_row<float, DB>(part + n, dv, h, a.D, fv);
         return;
     }
-    store_row<store_t<T>, DB>((store_t<T>*)a.dk + out_row * a.D, dk, h, a.D, a.scale);
-    store_row<store_t<T>, DB>((store_t<T>*)a.dv + out_row * a.D, dv, h, a.D, 1.f);
+    store_row<store_t<T>, DB>((store_t<T>*)a.dk + out_row * a.D, dk, h, a.D, fk);
+    store_row<store_t<T>, DB>((store_t<T>*)a.dv + out_row * a.D, dv, h, a.D, fv);
 }
 
 // dk and dv as the sums of their splits, in order

@@ -47,10 +47,59 @@ def test_visible_infinities_in_shares_of_no_weight(at, rows, keys, H, Hk, D, dt)
     assert torch.equal(out[rows:], clean[rows:]) and torch.equal(l2[rows:], lse[rows:])
 
 
-# ---- fp16: what lies below its normal range.  u = 2^-24.  A probability is rounded at 2^7 times its value relative to the row's maximum: half a step of fp16 of
-# itself (2^-11), and below the normal range half a subnormal step, 2^-25, of that: 2^-32 of the row's sum.
+# ---- fp16: what lies below its normal range.  u = 2^-24.  A probability is rounded at 2^7 (forward) and 2^12 (dv) times its value: half a step of fp16 of
+# itself (2^-11), and below the normal range half a subnormal step, 2^-25, of that: 2^-32 of the row's sum, 2^-37.  A ds is rounded at a power of two that brings
+# the largest so far of its row (dq) or key (dk) to 2^8 at least: 2^-11 of itself or 2^-33 of that largest one.  The other terms are those of
+# test_gpu_packed_attn.py: a score is off by es = (D + 8) u scale sum |q k| + 4 u |s|, a probability by 2 es + (nk + 36) u + 4 u |lse| of itself.
 U = 2.0 ** -24
 H16 = 2.0 ** -11
+
+
+def _grads16(q, k, v, g, scale, causal, o):
+    """one head, [n, D] each, o the forward pass' result in fp16 -> (out, tol), (dq, tol), (dk, tol), (dv, tol) in 64 bits"""
+    q, k, v, g, o16 = (t.double() for t in (q, k, v, g, o))
+    (a, D), b = q.shape, k.shape[0]
+    s = q @ k.t() * scale
+    if causal:
+        s = s.masked_fill(torch.ones(a, b, dtype=torch.bool, device="cuda").triu(b - a + 1), -math.inf)
+    es = ((D + 8) * U * scale * (q.abs() @ k.abs().t()) + 4 * U * s.abs().nan_to_num(posinf=0.0)).amax(1, keepdim=True)
+    lse, p = torch.logsumexp(s, 1, keepdim=True), torch.softmax(s, 1)
+    out, ep = p @ v, 2 * es + (b + 36) * U + 4 * U * lse.abs()
+    otol = (H16 + ep) * (p @ v.abs()) + b * 2.0 ** -32 * v.abs().amax(0) + H16 * out.abs() + 2.0 ** -25
+    dp, delta = g @ v.t(), (g * out).sum(1, keepdim=True)
+    edelta = (g.abs() * ((o16 - out).abs() + (D + 8) * U * out.abs())).sum(1, keepdim=True)   # the kernel takes the rounded output's
+    ds = p * (dp - delta)
+    eds = p * (ep * (dp - delta).abs() + (D + 8) * U * (g.abs() @ v.abs().t()) + edelta) + H16 * ds.abs()
+    low = 2.0 ** -33 * (ds.abs() + eds).amax(1, keepdim=True)
+    dq, tq = ds @ k * scale, scale * ((eds + low + (b + 32) * U * ds.abs()) @ k.abs())
+    low = 2.0 ** -33 * (ds.abs() + eds).amax(0, keepdim=True)
+    dk, tk = ds.t() @ q * scale, scale * ((eds + low + (a + 32) * U * ds.abs()).t() @ q.abs())
+    dv, tv = p.t() @ g, (p * (ep + H16 + (a + 32) * U) + 2.0 ** -37).t() @ g.abs()
+    fin = lambda x, t: (x, t + H16 * x.abs() + 2.0 ** -25)
+    return (out, otol), fin(dq, tq), fin(dk, tk), fin(dv, tv)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("rows,keys,causal", [(64, 4096, False), (33, 16384, False), (1500, 1500, True), (2, 9000, True)])
+@pytest.mark.parametrize("size,spread", [(1e-4, 1.0), (1e-3, 1.0), (100.0, 4.0), (6e4, 0.0)])
+def test_fp16_gradients_of_any_size(size, spread, rows, keys, causal, D):
+    """Gradients far below and above 1 (a mean over many tokens, a scaled loss), over keys that weigh 1 / nk and less: every ds and many
+    probabilities lie below fp16's normal range while the results lie in it."""
+    from casmtr_amd import ops
+    r = torch.Generator().manual_seed(rows + D)
+    q, k, v, g = (torch.randn(n, 2, D, generator=r) for n in (rows, keys, keys, rows))
+    g = g / g.abs().amax()
+    q, k, v, g = (t.half().cuda() for t in (q * spread / 16, k * 16, v, g * size))
+    cq, ck = cu([rows]), cu([keys])
+    out, lse = ops.packed_attn(q, k, v, cq, ck, causal=causal, want_lse=True)
+    got = (out, *ops.packed_attn_bwd(g, q, k, v, out, lse, cq, ck, causal=causal))
+    for h in (0, 1):
+        want = _grads16(q[:, h], k[:, h], v[:, h], g[:, h], D ** -0.5, causal, out[:, h])
+        for name, x, (ref, tol) in zip(("out", "dq", "dk", "dv"), got, want):
+            err = (x[:, h].double() - ref).abs()
+            over = err > tol
+            big = ref.abs() + tol > 65504.0          # (past the type's range: infinite)
+            assert not (over & ~big).any(), f"{name}: {(err / tol)[~big].max().item():.2f} of the tolerance"
 
 
 @pytest.mark.parametrize("D", [32, 64, 128])
