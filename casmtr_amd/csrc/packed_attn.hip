@@ -70,11 +70,12 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
     kv.of((const store_t<T>*)a.k + (long long)keys.begin * a.kts + hk * a.khs, (const store_t<T>*)a.v + (long long)keys.begin * a.vts + hk * a.vhs, keys.count);
     if (t0 < t1) kv.fetch(t0, 0);
     frag_t<T> qf[KS];
-    {
+    const auto load_q = [&](auto guard) {
         const store_t<T>* qr = (const store_t<T>*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = load_frag<T>(qr, s, h, a.D);
-    }
+        for (int s = 0; s < KS; ++s) qf[s] = load_frag<T, decltype(guard)::value>(qr, s, h, a.D);
+    };
+    load_q(std::false_type{});
     f32x16 acc[DB];
     float m, l;
     // One pass over the keys.  GUARD: with the product that keeps what a row does not see away from it (mma_hidden)
@@ -84,10 +85,11 @@ __global__ __launch_bounds__(64 * NW, !FEW && (sizeof(T) == 2 || (sizeof(T) == 1
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         m = -INFINITY;
         l = 0.f;
+        if (GUARD && std::is_same<T, x3_t>::value) load_q(guard);
         if (GUARD && t0 < t1) kv.fetch(t0, 0);   // (the first pass's first tile is under way)
         const auto step = [&](int t, auto stage_) {
             constexpr int stage = decltype(stage_)::value;   // a constant: it goes into the offsets of the LDS reads
-            kv.arrived(stage);
+            kv.template arrived<GUARD>(stage);
             __syncthreads();   // this tile is in LDS; nobody reads the other stage any more
             if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
             const int key0 = t * BN + wkey;

@@ -20,7 +20,8 @@ typedef u32x4 __attribute__((aligned(2))) u32x4_any;   // 16 bytes at any elemen
 
 // x3_t: fp32 data multiplied as three bf16 terms, x = x0 + x1 + x2 (8 bits each: the 24 bits of x), of whose nine products the six largest are
 // kept: what is dropped is below 2^-24 of the product, as the rounding of an fp32 product is.  Six bf16 matrix instructions of 32 cycles
-// stand for eight fp32 ones of 64.  (Values beyond 2^128 (1 - 2^-9) count as infinite.)
+// stand for eight fp32 ones of 64.  Magnitudes from 2^128 (1 - 2^-9) on round to an infinite x0; the products are not finite then, and the careful pass
+// (mma_any, mma_hidden) splits them the other way: x0 the largest bf16.
 struct x3_t {};
 template <typename T> struct FragOf { typedef T type __attribute__((ext_vector_type(8))); };
 template <> struct FragOf<x3_t> { struct type { FragOf<bf16_t>::type t[3]; }; };
@@ -49,7 +50,8 @@ __device__ __forceinline__ f32x16 mma(const frag_t<x3_t>& a, const frag_t<x3_t>&
     return mma(a.t[0], b.t[0], c);
 }
 // eight values in three terms, two at a time: one conversion to a packed pair, whose halves are the pair's values in fp32 with a shift and a mask
-// (11 instructions per pair; from single conversions the compiler makes 15)
+// (11 instructions per pair; from single conversions the compiler makes 15).  CAREFUL: the first term of a finite value is finite
+template <bool CAREFUL = false>
 __device__ __forceinline__ frag_t<x3_t> split3(const float (&x)[8]) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
@@ -59,7 +61,14 @@ __device__ __forceinline__ frag_t<x3_t> split3(const float (&x)[8]) {
         float u = x[2 * e], v = x[2 * e + 1];
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
-            const bf16x2 p = __builtin_convertvector(f32x2{u, v}, bf16x2);
+            f32x2 t = {u, v};
+            if constexpr (CAREFUL) {
+                const float top = __uint_as_float(0x7f7f0000u);   // the largest bf16
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (__builtin_fabsf(t[i]) < INFINITY) t[i] = __builtin_amdgcn_fmed3f(t[i], -top, top);
+            }
+            const bf16x2 p = __builtin_convertvector(t, bf16x2);
             __builtin_memcpy(&w[j][e], &p, 4);
             u -= __uint_as_float(w[j][e] << 16);
             v -= __uint_as_float(w[j][e] & 0xffff0000u);
@@ -176,7 +185,7 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int col, int D) {
     return r;
 }
 // the fragment of a row held in global memory: columns 16 s + 8 h ..
-template <typename T>
+template <typename T, bool CAREFUL = false>
 __device__ __forceinline__ frag_t<T> load_frag(const store_t<T>* row, int s, int h, int D) {
     frag_t<T> f;
     const int col = 16 * s + 8 * h;
@@ -185,7 +194,7 @@ __device__ __forceinline__ frag_t<T> load_frag(const store_t<T>* row, int s, int
         const u32x4 a = load_chunk(row, col, D), b = load_chunk(row, col + 4, D);
         __builtin_memcpy(x, &a, 16);
         __builtin_memcpy(x + 4, &b, 16);
-        f = split3(x);
+        f = split3<CAREFUL>(x);
     } else {
         const u32x4 a = load_chunk(row, col, D);
         __builtin_memcpy(&f, &a, 16);
@@ -275,6 +284,7 @@ struct TilePair {
             }
         }
     }
+    template <bool CAREFUL = false>
     __device__ __forceinline__ void arrived(int stage) {
         if constexpr (DMA) glds_wait<0>();
         else {
@@ -319,20 +329,22 @@ struct TilePair<x3_t, DP, ROWS, NW, false> {
             }
         }
     }
+    template <bool CAREFUL>
     static __device__ __forceinline__ void put(char* tile, int o, const u32x4& lo, const u32x4& hi) {
         float x[8];
         __builtin_memcpy(x, &lo, 16);
         __builtin_memcpy(x + 4, &hi, 16);
-        const frag_t<x3_t> f = split3(x);
+        const frag_t<x3_t> f = split3<CAREFUL>(x);
 #pragma unroll
         for (int j = 0; j < 3; ++j) *reinterpret_cast<frag_t<bf16_t>*>(tile + j * L::PLANE + o) = f.t[j];
     }
+    template <bool CAREFUL = false>
     __device__ __forceinline__ void arrived(int stage) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = tid + NT * i, o = P::off(id / P::CPR, id % P::CPR);
-            put(smem + 2 * stage * TB, o, ar[2 * i], ar[2 * i + 1]);
-            put(smem + (2 * stage + 1) * TB, o, br[2 * i], br[2 * i + 1]);
+            put<CAREFUL>(smem + 2 * stage * TB, o, ar[2 * i], ar[2 * i + 1]);
+            put<CAREFUL>(smem + (2 * stage + 1) * TB, o, br[2 * i], br[2 * i + 1]);
         }
     }
 };

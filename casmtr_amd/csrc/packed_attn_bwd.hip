@@ -115,14 +115,21 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <=
     const int t1 = (wg_end + BN - 1) / BN;
     const long long out_row = (long long)(rows.begin + tok) * a.H + head;
     frag_t<T> qf[KS], gf[KS];
+    const auto load_rows = [&](auto guard) {
+        const store_t<T>* qr = (const store_t<T>*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
+        const store_t<T>* gr = (const store_t<T>*)a.g + out_row * a.D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            qf[s] = load_frag<T, decltype(guard)::value>(qr, s, h, a.D);
+            gf[s] = load_frag<T, decltype(guard)::value>(gr, s, h, a.D);
+        }
+    };
+    load_rows(std::false_type{});
     float delta = 0.f;
     {
-        const store_t<T>* qr = (const store_t<T>*)a.q + (long long)(rows.begin + tok) * a.qts + head * a.qhs;
         const store_t<T> *gr = (const store_t<T>*)a.g + out_row * a.D, *orow = (const store_t<T>*)a.o + out_row * a.D;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            qf[s] = load_frag<T>(qr, s, h, a.D);
-            gf[s] = load_frag<T>(gr, s, h, a.D);
             float x[8], y[8];
             const int c = 16 * s + 8 * h, n = a.D - c;
 #pragma unroll
@@ -143,12 +150,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || (sizeof(T) == 1 && DP <=
     const auto pass = [&](auto guard) {
         constexpr bool GUARD = decltype(guard)::value;
         e = E_START;
+        if (GUARD && std::is_same<T, x3_t>::value) load_rows(guard);
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         if (0 < t1) kv.fetch(0, 0);
         const auto step = [&](int t, auto stage_) {
             constexpr int stage = decltype(stage_)::value;
-            kv.arrived(stage);
+            kv.template arrived<GUARD>(stage);
             __syncthreads();
             if (t + 1 < t1) kv.fetch(t + 1, stage ^ 1);
             if (t * BN >= wave_end) return;
@@ -223,15 +231,16 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
     const int first = first_of(key), wg_first = first_of(key0), wave_first = first_of(wk), wave_all = first_of(wk + 31);
     const int kc = max(0, min(key, keys.count - 1));
     frag_t<T> kf[KS], vf[KS];
-    {
+    const auto load_keys = [&](auto guard) {
         const store_t<T>* kr = (const store_t<T>*)a.k + (long long)(keys.begin + kc) * a.kts + hk * a.khs;
         const store_t<T>* vr = (const store_t<T>*)a.v + (long long)(keys.begin + kc) * a.vts + hk * a.vhs;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            kf[s] = load_frag<T>(kr, s, h, keys.count > 0 ? a.D : 0);
-            vf[s] = load_frag<T>(vr, s, h, keys.count > 0 ? a.D : 0);
+            kf[s] = load_frag<T, decltype(guard)::value>(kr, s, h, keys.count > 0 ? a.D : 0);
+            vf[s] = load_frag<T, decltype(guard)::value>(vr, s, h, keys.count > 0 ? a.D : 0);
         }
-    }
+    };
+    load_keys(std::false_type{});
     f32x16 dk[DB], dv[DB];
     int e = E_START;
     const int t0 = wg_first / BM, per = (rows.count + BM - 1) / BM - t0;   // tiles of a head
@@ -265,12 +274,13 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 && DP <= 64) || (sizeof(T)
 #pragma unroll
         for (int d = 0; d < DB; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
         e = E_START;
+        if (GUARD && std::is_same<T, x3_t>::value) load_keys(guard);
         if (n0 < turns) fetch(n0, 0);
         const auto step = [&](int n, auto stage_) {
             constexpr int stage = decltype(stage_)::value;
             const int t = t0 + n % per;
             if (tid < BM) { stat[stage][0][tid] = sl; stat[stage][1][tid] = sd; }
-            qg.arrived(stage);
+            qg.template arrived<GUARD>(stage);
             __syncthreads();
             if (n + 1 < turns) fetch(n + 1, stage ^ 1);
             if ((t + 1) * BM <= wave_first) return;

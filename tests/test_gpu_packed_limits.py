@@ -121,3 +121,48 @@ def test_fp16_many_small_probabilities(rows, keys, D):
             es = ((D + 8) * U * (q[:, 0].abs().double() @ k[:, 0].abs().double().t()) * 2).amax()
             tol = (2 * H16 + 2 * es + (keys + 32) * U) * ref + keys * 2.0 ** -32 * 1.5 + 2.0 ** -25
             assert ((out[:, 0].double() - ref).abs() <= tol).all(), ((out[:, 0].double() - ref).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 32), (2, 1, 64), (2, 2, 128)])
+@pytest.mark.parametrize("rows,keys", [(1, 300), (9, 100), (150, 300), (700, 90)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_largest_fp32_magnitudes(causal, rows, keys, H, Hk, D):
+    """The largest finite fp32 numbers are numbers on every path: keys of that magnitude meet zeros or numbers small enough, values of it weigh
+    nothing (their key's score is far below the others') or 2^-20.  Bounds as in test_gpu_packed_attn.py; scores are exact here but for (D + 8) u of what they add."""
+    from casmtr_amd import ops
+    top = torch.finfo(torch.float32).max
+    r = torch.Generator().manual_seed(rows)
+    q, k, v, g = (torch.randn(n, h, D, generator=r).cuda() for n, h in ((rows, H), (keys, Hk), (keys, Hk), (rows, H)))
+    cq, ck = cu([rows]), cu([keys])
+    q[..., 0], k[..., 0] = 0.0, 0.0
+    q[..., 1], k[..., 1] = 2.0 ** -126, 0.0
+    g[..., 2] = 0.0
+    for s in (1.0, -1.0):
+        k2, v2 = k.clone(), v.clone()
+        k2[1, :, 0], k2[3, :, 1] = s * top, -s * top    # meets 0; meets 2^-126: +-4 in the score
+        v2[5, :, 2] = s * top * 2.0 ** -20              # (weighs at most 1: well inside)
+        v2[6, :, 2], k2[6] = s * top, 0.0
+        k2[6, :, 3], q[..., 3] = -4000.0, 1.0           # weight exp(-4000 scale): nothing
+        o, lse = ops.packed_attn(q, k2, v2, cq, ck, causal=causal, scale=1.0, want_lse=True)
+        dq, dk, dv = ops.packed_attn_bwd(g, q, k2, v2, o, lse, cq, ck, causal=causal, scale=1.0)
+        assert o.isfinite().all() and dk.isfinite().all() and dv.isfinite().all()
+        for h in range(H):
+            m = h // (H // Hk)
+            Q, K, V, G = q[:, h].double(), k2[:, m].double(), v2[:, m].double(), g[:, h].double()
+            sc = Q @ K.t()
+            if causal:
+                sc = sc.masked_fill(torch.ones(rows, keys, dtype=torch.bool, device="cuda").triu(keys - rows + 1), -math.inf)
+            es = ((D + 8) * U * (Q.abs() @ K.abs().t()) + 4 * U * sc.abs()).masked_fill(sc == -math.inf, 0).masked_fill(sc < -3000, 0).amax(1, keepdim=True)
+            p = torch.softmax(sc, 1).nan_to_num(0.0)
+            lost = torch.where(p < 2.0 ** -125, p, 0.0)     # (the exponential gives 0 below the smallest normal number, 2^-126: such a p may go as a whole)
+            tol = (2 * es + (keys + 34) * U) * (p @ V.abs()) + lost @ V.abs() + 2.0 ** -149
+            assert ((o[:, h].double() - p @ V).abs() <= tol).all()
+            # dq: the 64-bit gradient within its bound, but where that passes fp32's range: |ds| above 1 times a key of the largest magnitude
+            dp, O = G @ V.t(), p @ V
+            delta = (G * O).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            ep = 2 * es + (keys + 36) * U + 4 * U * lse[:, h].double().abs().nan_to_num(posinf=0.0)[:, None]
+            eds = lost * (dp - delta).abs() + p * (ep * (dp - delta).abs() + (D + 8) * U * (G.abs() @ V.abs().t()) + (G.abs() * (tol + (D + 8) * U * O.abs())).sum(1, keepdim=True))
+            ref, tq = ds @ K, (eds + (keys + 32) * U * ds.abs()) @ K.abs()
+            fits = ref.abs() + tq + U * ref.abs() <= top
+            assert fits.double().mean() > 0.9 and ((dq[:, h].double() - ref).abs() <= tq + U * ref.abs())[fits].all()
