@@ -108,6 +108,18 @@ __device__ __forceinline__ float q8_scale(unsigned amax_bits, int quant) {
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;   // a row of zeros: the smallest normal number, whose reciprocal is finite (NaN stays)
 }
 
+// y / scale, correctly rounded but for quotients within 2^-46 of a border between two: the product with the reciprocal, which next to a border between
+// two codes is on the wrong side now and then, and one step with its remainder.  (16384 x 8192 into e4m3 with scales for 128 columns: the
+// division's own instructions 207 us, this 195, the product alone 191.)
+struct Quotient {
+    float sc, inv;   // sc: 0 for an infinite scale, which leaves the product (0, or NaN of an infinity) as it is
+    __device__ __forceinline__ explicit Quotient(float scale) : sc(scale < INFINITY ? scale : 0.f), inv(1.0f / scale) {}
+    __device__ __forceinline__ float operator()(float y) const {
+        const float q = y * inv;
+        return __builtin_fmaf(__builtin_fmaf(-q, sc, y), inv, q);
+    }
+};
+
 // TPR threads per row, CH chunks of 8 columns per thread: chunk i of thread t covers columns 8 (t + TPR i) .. + 7
 template <typename T, int TPR, int CH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
@@ -161,18 +173,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
         for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
         if (a.group) {    // 128 columns = the 16 chunks of one 16-lane row of the wave
             m = max(m, dpp_u32<0xB1>(m)); m = max(m, dpp_u32<0x4E>(m)); m = max(m, dpp_u32<0x141>(m)); m = max(m, dpp_u32<0x140>(m));
-            const float sc = q8_scale(m, a.quant), inv = 1.0f / sc;
+            const float sc = q8_scale(m, a.quant);
             if (n > 0) {
                 if ((t & 15) == 0) a.scale[row * (a.C / 128) + col / 128] = sc;
+                const Quotient by(sc);
                 float q[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) q[e] = v[i][e] * inv;
+                for (int e = 0; e < 8; ++e) q[e] = by(v[i][e]);
                 store_q8((unsigned char*)a.y + row * a.C + col, q, n, a.quant);
             }
         } else big = max(big, m);
     }
     if (!a.quant || a.group) return;
-    const float sc = q8_scale(row_max<TPR>(big, s_max), a.quant), inv = 1.0f / sc;
+    const float sc = q8_scale(row_max<TPR>(big, s_max), a.quant);
+    const Quotient by(sc);
     if (t == 0) a.scale[row] = sc;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -180,7 +194,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
         if (n <= 0) continue;
         float q[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = v[i][e] * inv;
+        for (int e = 0; e < 8; ++e) q[e] = by(v[i][e]);
         store_q8((unsigned char*)a.y + row * a.C + col, q, n, a.quant);
     }
 }
