@@ -126,6 +126,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
     constexpr int RPW = TPR < 256 ? 256 / TPR : 1;
     __shared__ float s_sum[TPR < 256 ? 1 : TPR / 64];
     __shared__ unsigned s_max[TPR < 256 ? 1 : TPR / 64];
+    __shared__ float s_big[TPR < 256 ? 1 : TPR / 64];
     const int t = threadIdx.x % TPR;
     const long long row = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RPW + threadIdx.x / TPR;
     if (row >= a.rows) return;   // whole waves only where a row is a wave's, the whole workgroup never otherwise
@@ -152,7 +153,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
         for (int e = 0; e < 8; ++e) s = fmaf(v[i][e], v[i][e], s);
     }
     s = row_add<TPR>(s, s_sum);
-    const float rstd = 1.0f / sqrtf(s * a.inv_c + a.eps);
+    float rstd = 1.0f / sqrtf(s * a.inv_c + a.eps);
+    if (!(s < INFINITY)) {   // (the same for the whole row) squares past fp32, from |h| = 1.8e19 on: of 2^-80 h, beside which eps is nothing
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(v[i][e] * 0x1p-80f, v[i][e] * 0x1p-80f, s);
+        rstd = 0x1p-80f / sqrtf(row_add<TPR>(s, s_big) * a.inv_c);
+    }
     if (a.rstd && t == 0) a.rstd[row] = rstd;
     unsigned big = 0;
 #pragma unroll

@@ -35,3 +35,30 @@ def test_codes(C, group, q8):
         want = (sign * y / s).clamp(-TOP[q8], TOP[q8])              # one correctly rounded division
         want = want.round() if q8 == torch.int8 else want.to(q8).float()
         assert torch.equal(q.float().cpu(), want.expand(3, C))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("R,C", [(3, 64), (2, 1000), (3, 4096), (2, 16384)])
+@pytest.mark.parametrize("size", [1e20, 1e30, 1e38])
+def test_rows_whose_squares_pass_fp32(size, R, C, dt):
+    """The norm of large rows: their squares do not fit fp32, the result does.  rstd may be subnormal (a row of 1e38: 1e-38 and less, of steps of
+    2^-149): 2^-22 of itself, beside the 32 u that the sums, the root and the products are off by.  Ordinary rows beside them keep their bits."""
+    from casmtr_amd import ops
+    u = 2.0 ** -24
+    g = torch.Generator().manual_seed(C)
+    x = torch.rand(R, C, generator=g) * 2.0 + 0.5
+    x = torch.where(torch.rand(R, C, generator=g) < 0.5, -x, x).to(dt).cuda()
+    w = (1 + 0.3 * torch.randn(C, generator=g)).cuda()
+    big = x.clone()
+    big[0] = (x[0].double() * size).to(dt)
+    y, _, rstd = ops.rms_norm(big, w, 1e-5, want_rstd=True)
+    h = big[0].double()
+    ref = h / (h.square().mean() + 1e-5).sqrt() * w.double()
+    assert ((y[0].double() - ref).abs() <= (torch.finfo(dt).eps / 2 + 32 * u + 2.0 ** -21) * ref.abs()).all()
+    assert torch.equal(y[1:], ops.rms_norm(x, w, 1e-5)[0][1:])
+    dy = torch.randn(R, C, generator=g).to(dt).cuda()
+    dx, dw = ops.rms_norm_bwd(dy, big, w, rstd)
+    n = big.double() / (big.double().square().mean(1, keepdim=True) + 1e-5).sqrt()
+    terms = dy.double() * n
+    assert ((dw.double() - terms.sum(0)).abs() <= (140 * u + 2.0 ** -21) * terms.abs().sum(0) + u * terms.sum(0).abs()).all()
+    assert (dx[0].double().abs() * size <= 40.0).all() and dx.isfinite().all()
