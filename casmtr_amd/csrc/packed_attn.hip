@@ -29,7 +29,7 @@ struct AttnArgs {
     float scale;                       // times log2(e): scores are in bits
 };
 
-constexpr float LN2 = 0.693147180559945309f;
+constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float RESCALE_AT = 8.f;   // the accumulator is rescaled only when a maximum grew by more than 8 bits: exp2 stays below 256, far from any overflow
 // Probabilities are multiplied as 2^P_BITS of their value: in fp16 they stay in the normal range down to 2^-21 of the row's largest then, and what is lost
 // below that is at most 2^-32 of it each -- beside 2^-25 without, which 65536 keys of 2^-25 make up to a whole result.  2^(RESCALE_AT + 7) is within
@@ -345,7 +345,7 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
                                       const int* len_k, long long Tq, long long Tk, int nseq, int H, int Hk, int D, long long qts, long long qhs,
                                       long long kts, long long khs, long long vts, long long vhs, float scale, int causal, int dtype,
                                       casmtr_stream_t stream) {
-    if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale < INFINITY) ||
+    if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale * LOG2E < INFINITY) ||
         Tq > 0x7fffff00LL || Tk > 0x7fffff00LL || Tq * (H / Hk) > 0x7fffff00LL)
         return CASMTR_ERR_UNSUPPORTED;
     if (Tq == 0) return 0;
@@ -355,7 +355,7 @@ extern "C" int casmtr_packed_attn_fwd(const void* q, const void* k, const void* 
     const long long rows = Tq * H, wgs = slot_count(Tq, G, nseq, few || one ? 32 : 32 * FWD_NW) * Hk;
     if (wgs > 0x7fffffffLL) return CASMTR_ERR_UNSUPPORTED;
     AttnArgs a{q, k, v, o, lse, ws, ws ? ws + (long long)splits * rows * D : nullptr, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk},
-               qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits, scale * 1.44269504088896341f};
+               qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits, scale * LOG2E};
     ProfScope ps(CASMTR_PROF_GLUE, (hipStream_t)stream, "packed_attn_kernel");
     const bool ok = with_type(dtype, [&](auto tv) {
         typedef decltype(tv) T;

@@ -406,14 +406,14 @@ extern "C" int casmtr_packed_attn_bwd(const void* g, const void* q, const void* 
                                       void* dv, float* ws, const int* cu_q, const int* cu_k, const int* len_k, long long Tq, long long Tk, int nseq,
                                       int H, int Hk, int D, long long qts, long long qhs, long long kts, long long khs, long long vts, long long vhs,
                                       float scale, int causal, int dtype, casmtr_stream_t stream) {
-    if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale < INFINITY) ||
+    if (Tq < 0 || Tk < 0 || nseq < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128 || !(scale > 0.f) || !(scale * LOG2E < INFINITY) ||
         Tq > 0x7fffff00LL || Tk > 0x7fffff00LL || Tq * (H / Hk) > 0x7fffff00LL || dtype < 0 || dtype > CASMTR_BF16)
         return CASMTR_ERR_UNSUPPORTED;
     if (Tq == 0 && Tk == 0) return 0;
     const int G = H / Hk;
     const long long qwgs = slot_count(Tq, G, nseq, 32 * BWD_NW) * Hk, kwgs = slot_count(Tk, 1, nseq, 32 * BWD_NW) * Hk;
     if (qwgs > 0x7fffffffLL || kwgs > 0x7fffffffLL) return CASMTR_ERR_UNSUPPORTED;
-    if (Tq > 0 && !ws) return CASMTR_ERR_UNSUPPORTED;
+    if (Tq > 0 && (!ws || !lse)) return CASMTR_ERR_UNSUPPORTED;
     const int splits = Tq > 0 ? split_rows(Tk, nseq, Hk) : 1;
     float* part = ws ? ws + (((size_t)Tq * H + 3) & ~(size_t)3) : nullptr;
     BwdArgs a{q, k, v, o, g, lse, ws, part, dq, dk, dv, {cu_q, cu_k, len_k, nseq, G, causal != 0, Tq, Tk}, qts, qhs, kts, khs, vts, vhs, H, Hk, D, splits,

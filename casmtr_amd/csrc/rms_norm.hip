@@ -352,7 +352,7 @@ extern "C" size_t casmtr_rms_norm_bwd_ws_floats(long long rows, int C) { return 
 extern "C" int casmtr_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* ws,
                                    long long rows, int C, long long dy_stride, long long dh_stride, long long h_stride, int dtype, int w_dtype,
                                    casmtr_stream_t stream) {
-    if (rows <= 0 || C <= 0 || rows > 0x7fffffffLL || (w_dtype != CASMTR_F32 && w_dtype != dtype)) return CASMTR_ERR_UNSUPPORTED;
+    if (rows <= 0 || C <= 0 || rows > 0x7fffffffLL || !rstd || !ws || (w_dtype != CASMTR_F32 && w_dtype != dtype)) return CASMTR_ERR_UNSUPPORTED;
     NormBwdArgs a{dy, dh, h, w, rstd, dx, ws, rows, dy_stride, dh_stride, h_stride, C, w_dtype == CASMTR_F32, 1.0f / (float)C};
     const int parts = bwd_parts(rows, C);
     bool ok = false;

@@ -348,9 +348,10 @@ int casmtr_rotary_fwd(const void* q, const void* k, const void* pos, const doubl
  * len_k[s] (a cache of fixed shares).  cu_q, cu_k [nseq+1], len_k [nseq] int32 on the device, non-decreasing; they are read by the
  * kernels alone, which stay inside the tensors whatever they hold.
  *   o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j),  lse_i = log sum_j exp(scale q_i . k_j)      (lse [Tq,H] fp32 or NULL)
- * (fp32 products are made of bf16 terms that carry all 24 bits: accurate as fp32, but not its bits)  over all keys of the sequence, or, causal, those with j <= i + nk - nq (the last row sees every key).  A row that sees no key, and a
- * row outside every sequence, gives 0 and -inf.  Infinities and NaN in keys and values reach the rows that see them and no others.
- * scale > 0.  ws: casmtr_packed_attn_ws_floats() floats (0: none needed).                                                       */
+ * over all keys of the sequence, or, causal, those with j <= i + nk - nq (the last row sees every key).  A row that sees no key, and a row
+ * outside every sequence, gives 0 and -inf.  Infinities and NaN in keys and values reach the rows that see them and no others.  fp32 products are
+ * made of bf16 terms that carry all 24 bits: accurate as fp32, but not its bits.  0 < scale < 2^127.
+ * ws: casmtr_packed_attn_ws_floats() floats (0: none needed).                                                                   */
 size_t casmtr_packed_attn_ws_floats(long long Tq, long long Tk, int nseq, int H, int Hk, int D);
 int casmtr_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, float* ws, const int* cu_q, const int* cu_k,
                            const int* len_k, long long Tq, long long Tk, int nseq, int H, int Hk, int D, long long q_token_stride,
