@@ -85,3 +85,18 @@ def test_norm_gradient_of_many_rows(R, C, dt):
     adds = -(-R // parts) + -(-parts // 32) + 32
     want = terms.sum(0)
     assert ((dw.double() - want).abs() <= half(dt) * want.abs() + (adds + 36) * U * terms.abs().sum(0) + sub(dt)).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 128), (6, 2, 32), (4, 4, 64)])
+def test_prompts_beside_single_tokens(H, Hk, D, dt):
+    """a serving batch in one call: a whole prompt, parts of prompts behind what their caches hold, single tokens over long and short caches"""
+    from casmtr_amd import ops
+    cap, lens = 3000, [(1, 2999), (700, 700), (1, 5), (300, 2500), (1, 3000), (0, 90), (1, 1), (17, 1400), (1, 0)]
+    q, k, v, cq, _ = make([(a, cap) for a, _ in lens], H, Hk, D, dt, tail=0)
+    for s, (_, n) in enumerate(lens):
+        k[s * cap + n:(s + 1) * cap], v[s * cap + n:(s + 1) * cap] = float("nan"), float("inf")
+    ln = torch.tensor([n for _, n in lens], dtype=torch.int32).cuda()
+    for causal in (False, True):
+        out, lse = ops.packed_attn(q, k, v, cq, cu([cap] * len(lens)), len_k=ln, causal=causal, want_lse=True)
+        check(out, lse, reference(q, k, v, lens, causal, D ** -0.5, starts=[s * cap for s in range(len(lens))]))
