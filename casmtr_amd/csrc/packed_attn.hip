@@ -3,8 +3,8 @@
 // Row i of a sequence with nq rows and nk keys sees all keys, or, causal, the keys j <= i + nk - nq.  A row that sees none gives 0 and -inf.
 // Query heads share key heads in groups of G = H / Hk.
 //
-// fp32 runs as three bf16 terms (x3_t) -- 8 x 43264 rows x 676 keys, 4 heads of 32: 0.76 to 0.80 ms (150 TFLOP/s and more) against 1.12 ms on the fp32 matrix
-// instructions, whose 154 TFLOP/s bound it --, except for few rows, where the reads bound it.
+// fp32 runs as three bf16 terms (x3_t) -- 8 x 43264 rows x 676 keys, 4 heads of 32: 0.76 ms in a row of calls, 0.83 in a kernel trace of five (158 and 145
+// TFLOP/s) against 1.12 ms on the fp32 matrix instructions, whose 154 TFLOP/s bound it --, except for few rows, where the reads bound it.
 //
 // One pass over the keys with the running maximum and sum of the softmax.  A tile's rows are (token, head of the group) pairs, token-major, so
 // all G heads of a key head use one copy of its keys, and a single token of G heads is one tile.  A workgroup has four waves of 32 rows; K and V
@@ -12,7 +12,8 @@
 // Bound by the matrix instructions (heads of 128: 53 % of the cycles are theirs at the clock that they leave, 1.8 GHz) and, for smaller heads, by the
 // exponentials: 32 of 16 cycles each beside 512 cycles of matrix instructions per tile of 64 keys and wave at 64 columns.  So registers are kept
 // to two (64 and less: three) waves per SIMD that take turns; with two, heads of 64 ran at 752 in place of 860 TFLOP/s.  16384 causal tokens,
-// 32 / 8 heads of 128, fp16: 2.1 ms, 1.0 PFLOP/s (a library product of 8192^3: 1.05).  LDS conflicts: none.
+// 32 / 8 heads of 128: bf16 2.16 ms (1.02 PFLOP/s), fp16 2.21 (0.99; a library product of 8192^3: 1.05), the first calls on a cold card up to 2.45.
+// LDS conflicts: none.
 #include "packed_attn.hpp"
 
 using namespace casmtr;

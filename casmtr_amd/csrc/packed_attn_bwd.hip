@@ -4,11 +4,12 @@
 // No atomics: one kernel owns query rows and walks the keys (dq, and delta on the way), one owns keys and walks the query rows of all
 // heads that share them (dk, dv: the sum over the group is in the accumulator; in parts that a third kernel adds where there are few keys).  The scores are computed twice for it -- 7 products
 // instead of 5 -- and results repeat bit for bit.  Bound by the matrix instructions and, for heads of 64 and less, the exponentials beside them.
-// 16384 causal tokens, bf16: 32 / 8 heads of 128 dq 2.79 ms (1.18 PFLOP/s), dk and dv 5.03 ms (0.87; one wave per SIMD: K, V and both sums take 440
-// registers); 16 heads of 64 dq 0.78 ms (1.06), dk and dv 1.13 ms (0.98).
+// 16384 causal tokens, bf16: 32 / 8 heads of 128 dq 2.87 ms (1.15 PFLOP/s), dk and dv 5.6 ms (0.78; one wave per SIMD: K, V and both sums take 435
+// registers); 16 heads of 64 dq 0.79 ms (1.05), dk and dv 1.12 ms (0.98).
 // Roundings to 16 bits: p and ds, for the products with them.  In fp16 at a power of two that keeps them in its normal range: p (at most 1, the smaller
 // the more keys there are) at 2^12, ds, whose size follows the gradient's, at a running one (in_range).  Unscaled, gradients of 1e-3 over
-// 4096 keys lost most of their bits on the way to dq and dk.
+// 4096 keys lost most of their bits on the way to dq and dk.  It costs the largest and a product per element: the same sizes in fp16 take dq 3.18, dk and dv
+// 5.7 ms; 0.92 and 1.26 ms.
 #include "packed_attn.hpp"
 
 using namespace casmtr;
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_join_kernel(const BwdArgs
 constexpr int BWD_NW = 4;
 
 // Parts that the rows of a key tile are split into.  A key tile walks all rows of all the heads that share it, so few key heads leave the chip to
-// a few long workgroups; each part costs a write and a read of dk and dv in fp32.  6 packed documents up to 4096, 4 key heads of 64, 372 key
+// a few long workgroups; each part costs a write and a read of dk and dv in fp32.  6 packed documents up to 4096, 4 key heads of 64, 432 key
 // tiles, both kernels with parts for at least 512 / 768 / 1024 / 1400 / 2048 workgroups: 346 / 339 / 307 / 327 / 316 us.
 int split_rows(long long Tk, int n, int Hk) {
     const long long wgs = slot_count(Tk, 1, n, 32 * BWD_NW) * Hk;

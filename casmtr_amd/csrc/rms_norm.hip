@@ -6,7 +6,7 @@
 // Bound by HBM: a row is read once, kept in registers (CH chunks of 8 elements per thread) between the sum of squares and the output,
 // and everything a row needs is one launch.  A row belongs to one wave up to 1024 columns (the reduction is 6 DPP steps, no barrier),
 // to a workgroup of 256 threads up to 8192, of 1024 threads up to 16384 (with 256 the gradient's kernel needs 284 registers per thread).
-// 8192 x 4096 bf16 with residual 46.5 us (5.8 TB/s); 16384 x 8192 into e4m3 with scales for 128 columns 177 us (5.3 TB/s).
+// 8192 x 4096 bf16 with residual 50 us (41 to 52, 5.4 TB/s); 16384 x 8192 into e4m3 with scales for 128 columns 179 us (5.2 TB/s).
 // Sums are fp32 in a fixed order; the weight's gradient is reduced without atomics (per-workgroup partial sums in the workspace, then one
 // column-wise pass), so results repeat bit for bit.
 #include "token_types.hpp"
@@ -109,7 +109,7 @@ __device__ __forceinline__ float q8_scale(unsigned amax_bits, int quant) {
 }
 
 // y / scale, correctly rounded but for quotients within 2^-46 of a border between two: the product with the reciprocal, which next to a border between
-// two codes is on the wrong side now and then, and one step with its remainder.  (16384 x 8192 into e4m3 with scales for 128 columns: the
+// two codes is on the wrong side now and then, and one step with its remainder.  (16384 x 8192 into e4m3 with scales for 128 columns, call by call: the
 // division's own instructions 207 us, this 195, the product alone 191.)
 struct Quotient {
     float sc, inv;   // sc: 0 for an infinite scale, which leaves the product (0, or NaN of an infinity) as it is

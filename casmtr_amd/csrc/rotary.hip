@@ -6,7 +6,7 @@
 // Bound by HBM: every element is read and written once.  The angle is reduced in 64 bits (t / 2 pi minus the nearest whole number: at
 // position 10^6 a product in 32 bits is off by 0.03 rad) and the sine and cosine are taken of the remainder, once per token and pair for
 // all heads: a workgroup puts the table of its tokens in LDS, then streams the heads, eight pairs (two 16-byte vectors of 16-bit
-// data) per thread and step.  16384 tokens x 40 heads of 128, bf16: 71 to 74 us, 4.6 TB/s.
+// data) per thread and step.  16384 tokens x 40 heads of 128, bf16: 71 to 79 us, 4.7 to 4.2 TB/s.
 #include "token_types.hpp"
 
 using namespace casmtr;

@@ -865,8 +865,9 @@ def rotary_freqs(dim, base=10000.0, factor=1.0, trained=None, axes=1, device="cu
     the column of an image token.  Pair i of an axis' n turns by position * base^(-i / n).
     factor > 1 stretches the positions for contexts `factor` times longer than trained:
       trained=None     every frequency is divided by the factor (linear interpolation of positions), gain 1
-      trained=length   frequencies with more than 32 turns over the trained length stay, those with less than one are divided by the
-                       factor, in between they are blended linearly in the number of turns; gain 0.1 ln(factor) + 1"""
+      trained=length   the published YaRN scheme (Peng et al., 2023) with its bounds of 1 and 32: frequencies with more than 32 turns over the
+                       trained length stay, those with less than one are divided by the factor, in between they are blended linearly
+                       in the number of turns; gain 0.1 ln(factor) + 1"""
     if dim <= 0 or axes not in (1, 2) or dim % (2 * axes):
         raise RuntimeError(f"rotary_freqs: dim must be a positive multiple of 2 * axes and axes 1 or 2, got dim {dim}, axes {axes}")
     if not base > 0 or not factor >= 1 or (trained is not None and not trained > 0):
@@ -962,8 +963,9 @@ def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, 
     cu_k = 0, capacity, 2 capacity, ... and len_k the tokens so far is the form for single tokens; the keys are then split over workgroups.
     causal: row i sees the keys j <= i + nk - nq.  A row that sees no key, or belongs to no sequence, gives 0 (lse -inf).  What lies behind
     a sequence's keys is never read into a result, and infinities or NaN in keys and values reach only the rows that see them.
-    Scores, softmax statistics and sums are fp32; probabilities are rounded to the values' type for the product with them.  No host
-    synchronisation; safe to capture into a HIP graph."""
+    Scores, softmax statistics and sums are fp32; probabilities are rounded to the values' type for the product with them (fp16: at 2^7 of their
+    value, so that what falls below its normal range is at most 2^-32 of the row's largest).  No host synchronisation; safe to capture
+    into a HIP graph."""
     cu_k, scale, sizes, strides = _packed_args(q, k, v, cu_q, cu_k, len_k, scale)
     dev, dt = q.device, q.dtype
     out = q.new_empty(q.shape)
@@ -980,7 +982,8 @@ def packed_attn(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None, 
 
 def packed_attn_bwd(grad, q, k, v, out, lse, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
     """Gradient of packed_attn: grad like out (contiguous), out and lse as the forward pass returned them -> (dq, dk, dv), contiguous; dk and dv
-    sum over the heads that share a key head.  No atomics: the same call gives the same bits."""
+    sum over the heads that share a key head.  No atomics: the same call gives the same bits.  p and ds are rounded to q's type for the products
+    with them, in fp16 at powers of two that keep them in its normal range, so the gradient may be of any size."""
     cu_k, scale, sizes, strides = _packed_args(q, k, v, cu_q, cu_k, len_k, scale)
     Tq, Tk, n, H, Hk, D = sizes
     for t, name, shape, dtype in ((grad, "grad", (Tq, H, D), q.dtype), (out, "out", (Tq, H, D), q.dtype), (lse, "lse", (Tq, H), torch.float32)):
